@@ -45,7 +45,7 @@ def build_runtime(force: bool = False, verbose_ptxas: bool = False) -> str:
         return LIB
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     srcs = [os.path.join(CSRC, "frisk_b200.cu"), os.path.join(CSRC, "reduce.cu"),
-            os.path.join(CSRC, "layout_map.cpp")]
+            os.path.join(CSRC, "quant.cu"), os.path.join(CSRC, "layout_map.cpp")]
     cmd = [nvcc, *NVCC_FLAGS, "-shared", "-o", LIB, *srcs, "-lcudart"]
     if verbose_ptxas:
         cmd[1:1] = ["-Xptxas", "-v"]

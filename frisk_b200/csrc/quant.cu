@@ -1,0 +1,201 @@
+// Host side of the 8-bit row makers: argument checks, launches, and the C ABI entry points declared
+// in include/frisk_b200.h.
+#include "quant.cuh"
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include <string>
+
+#include "../../include/frisk_b200.h"
+#include "abi_internal.h"
+
+namespace {
+
+using frisk_quant::Params;
+
+int in_bytes(int dt) { return dt == FRISK_DT_F32 ? 4 : (dt == FRISK_DT_F16 || dt == FRISK_DT_BF16) ? 2 : 0; }
+bool is_8bit(int dt) { return dt == FRISK_DT_I8 || dt == FRISK_DT_E4M3 || dt == FRISK_DT_E5M2; }
+
+int fail(int code, const char* text) {
+  frisk_internal_set_error(text);
+  return code;
+}
+int fail_cuda(cudaError_t e, const char* what) {
+  frisk_internal_set_error((std::string(what) + ": " + cudaGetErrorString(e)).c_str());
+  return FRISK_ERR_CUDA;
+}
+
+int check_desc(const frisk_quant_desc& d) {
+  if (d.rows < 0 || d.cols <= 0) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: rows must not be negative, cols must be positive");
+  if (d.kind < FRISK_QUANT_PLAIN || d.kind > FRISK_QUANT_SILU_MUL) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: unknown kind");
+  if (!in_bytes(d.in_type)) return fail(FRISK_ERR_UNSUPPORTED, "quant: the input type must be f32, f16 or bf16");
+  if (!is_8bit(d.q_type)) return fail(FRISK_ERR_UNSUPPORTED, "quant: the output type must be i8, e4m3 or e5m2");
+  if (d.kind == FRISK_QUANT_RMSNORM) {
+    if (d.weight_type != d.in_type && d.weight_type != FRISK_DT_F32)
+      return fail(FRISK_ERR_UNSUPPORTED, "quant: the weight's type must be the input's or f32");
+    if (!(d.eps >= 0.f) || std::isinf(d.eps)) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: eps must be finite and not negative");
+  }
+  // rows and pitches below 2^40 keep every product of the two, in bytes, inside 64 bits
+  const int64_t lim = 1ll << 40;
+  if (d.rows >= lim || d.cols >= (1ll << 31) || d.ldx >= lim || d.ldo >= lim || d.lds >= lim || d.ldq >= lim)
+    return fail(FRISK_ERR_TOO_LARGE, "quant: 2^31 columns or more, or rows or pitches of 2^40 or more");
+  // (silu_mul with gate and up in one buffer needs 2 * cols; checked when the pointers are known)
+  if ((d.ldx && d.ldx < d.cols) || (d.ldo && d.ldo < d.cols) || (d.lds && d.lds < d.cols) || (d.ldq && d.ldq < d.cols))
+    return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: a pitch is shorter than a row");
+  return FRISK_OK;
+}
+
+template <typename TIn, typename TW, int QT, int KIND>
+cudaError_t launch(const Params& p, int64_t ctas, cudaStream_t st) {
+  frisk_quant::quant_rows_generic_kernel<TIn, TW, QT, KIND><<<(unsigned)ctas, 256, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename TIn, int QT>
+cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, cudaStream_t st) {
+  const int64_t ctas = std::min<int64_t>(d.rows, 0x7fffffff);
+  switch (d.kind) {
+    case FRISK_QUANT_PLAIN: return launch<TIn, TIn, QT, FRISK_QUANT_PLAIN>(p, ctas, st);
+    case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, QT, FRISK_QUANT_SILU_MUL>(p, ctas, st);
+    default:
+      return d.weight_type == d.in_type ? launch<TIn, TIn, QT, FRISK_QUANT_RMSNORM>(p, ctas, st)
+                                        : launch<TIn, float, QT, FRISK_QUANT_RMSNORM>(p, ctas, st);
+  }
+}
+
+template <typename TIn>
+cudaError_t launch_q(const frisk_quant_desc& d, const Params& p, cudaStream_t st) {
+  switch (d.q_type) {
+    case FRISK_DT_I8: return launch_kind<TIn, FRISK_DT_I8>(d, p, st);
+    case FRISK_DT_E4M3: return launch_kind<TIn, FRISK_DT_E4M3>(d, p, st);
+    default: return launch_kind<TIn, FRISK_DT_E5M2>(d, p, st);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* args) {
+  if (!desc || !args) return FRISK_ERR_INVALID_ARGUMENT;
+  const frisk_quant_desc& d = *desc;
+  if (int rc = check_desc(d)) return rc;
+  const bool norm = d.kind == FRISK_QUANT_RMSNORM, gated = d.kind == FRISK_QUANT_SILU_MUL;
+  if ((!norm && (args->residual || args->weight || args->sum_out)) || (!gated && args->up))
+    return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: an operand that this kind does not take was given");
+  if (args->sum_out && !args->residual) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: sum_out without a residual");
+  Params p{};
+  p.rows = d.rows;
+  p.cols = d.cols;
+  const bool halves = gated && !args->up;   // gate and up side by side in one buffer
+  p.ldx = d.ldx ? d.ldx : (halves ? 2 : 1) * d.cols;
+  if (halves && p.ldx < 2 * d.cols) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: a pitch is shorter than gate and up together");
+  p.ldo = halves ? p.ldx : d.ldo ? d.ldo : d.cols;
+  p.lds = d.lds ? d.lds : d.cols;
+  p.ldq = d.ldq ? d.ldq : d.cols;
+  p.eps = d.eps;
+  if (d.rows == 0) return FRISK_OK;
+  if (!args->x || !args->q || !args->scale) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: null x, q or scale");
+  const int es = in_bytes(d.in_type), ws = in_bytes(norm ? d.weight_type : d.in_type);
+  p.x = args->x;
+  p.other = norm ? args->residual : halves ? static_cast<const char*>(args->x) + d.cols * es : args->up;
+  p.weight = args->weight;
+  p.sum_out = args->sum_out;
+  p.q = args->q;
+  p.scale = args->scale;
+  auto off = [](const void* ptr, int a) { return reinterpret_cast<uintptr_t>(ptr) % (unsigned)a != 0; };
+  if (off(p.x, es) || off(p.other, es) || off(p.weight, ws) || off(p.sum_out, es) || off(p.scale, 4))
+    return fail(FRISK_ERR_MISALIGNED, "quant: a pointer is not aligned to its element size");
+  // the sum may replace x or the residual, element for element
+  if ((p.sum_out == p.x && p.sum_out && p.lds != p.ldx) || (p.sum_out == p.other && p.sum_out && p.lds != p.ldo))
+    return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: sum_out in place of x or the residual needs the same pitch");
+  int prev = -1;
+  cudaError_t e;
+  if (d.device >= 0) {
+    if ((e = cudaGetDevice(&prev)) != cudaSuccess) return fail_cuda(e, "cudaGetDevice");
+    if (prev != d.device && (e = cudaSetDevice(d.device)) != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
+  switch (d.in_type) {
+    case FRISK_DT_F32: e = launch_q<float>(d, p, st); break;
+    case FRISK_DT_F16: e = launch_q<__half>(d, p, st); break;
+    default: e = launch_q<__nv_bfloat16>(d, p, st); break;
+  }
+  if (prev >= 0 && prev != d.device) cudaSetDevice(prev);
+  if (e != cudaSuccess) return fail_cuda(e, "quant kernel launch");
+  return FRISK_OK;
+}
+
+int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_args* args) {
+  if (!desc || !args) return FRISK_ERR_INVALID_ARGUMENT;
+  frisk_quant_desc d = *desc;
+  if (int rc = check_desc(d)) return rc;
+  if (d.rows == 0) return FRISK_OK;
+  if (!args->x || !args->q || !args->scale) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: null x, q or scale");
+  const bool norm = d.kind == FRISK_QUANT_RMSNORM, gated = d.kind == FRISK_QUANT_SILU_MUL;
+  const int es = in_bytes(d.in_type);
+  // only the elements of each row travel: a host buffer may end behind the last row's
+  const int64_t xw = (gated && !args->up ? 2 : 1) * d.cols;
+  if (d.ldx && d.ldx < xw) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: a pitch is shorter than gate and up together");
+  struct Buf {
+    void* dev;
+    const void* in;   // host source, or nullptr
+    void* out;        // host destination, or nullptr
+    int64_t ld, width, rows;
+    int es;
+  };
+  const void* other = norm ? args->residual : gated ? args->up : nullptr;
+  enum { X, O, Wt, S, Q, Sc, N };
+  Buf b[N] = {
+      {nullptr, args->x, nullptr, d.ldx ? d.ldx : xw, xw, d.rows, es},
+      {nullptr, other, nullptr, d.ldo ? d.ldo : d.cols, d.cols, d.rows, es},
+      {nullptr, norm ? args->weight : nullptr, nullptr, d.cols, d.cols, 1, norm ? in_bytes(d.weight_type) : es},
+      {nullptr, nullptr, norm ? args->sum_out : nullptr, d.lds ? d.lds : d.cols, d.cols, d.rows, es},
+      {nullptr, nullptr, args->q, d.ldq ? d.ldq : d.cols, d.cols, d.rows, 1},
+      {nullptr, nullptr, args->scale, 1, 1, d.rows, 4},
+  };
+  int prev = -1;
+  cudaError_t e = cudaSuccess;
+  if (d.device >= 0) {
+    if ((e = cudaGetDevice(&prev)) != cudaSuccess) return fail_cuda(e, "cudaGetDevice");
+    if (prev != d.device && (e = cudaSetDevice(d.device)) != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
+  }
+  cudaStream_t st = nullptr;
+  e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  for (Buf& u : b) {   // packed on the device
+    if (e != cudaSuccess || (!u.in && !u.out)) continue;
+    e = cudaMalloc(&u.dev, (size_t)u.rows * u.width * u.es);
+    if (e == cudaSuccess && u.in)
+      e = cudaMemcpy2DAsync(u.dev, u.width * u.es, u.in, u.ld * u.es, u.width * u.es, u.rows, cudaMemcpyHostToDevice, st);
+  }
+  int rc = FRISK_OK;
+  if (e == cudaSuccess) {
+    frisk_quant_args a = *args;
+    a.x = b[X].dev;
+    if (norm) a.residual = b[O].dev;
+    if (gated) a.up = b[O].dev;
+    if (norm) a.weight = b[Wt].dev;
+    if (norm) a.sum_out = b[S].dev;
+    a.q = b[Q].dev;
+    a.scale = static_cast<float*>(b[Sc].dev);
+    a.stream = st;
+    d.ldx = d.ldo = d.lds = d.ldq = 0;
+    d.device = -1;
+    rc = frisk_b200_quant_run(&d, &a);
+    for (Buf& u : b)
+      if (rc == FRISK_OK && e == cudaSuccess && u.out)
+        e = cudaMemcpy2DAsync(u.out, u.ld * u.es, u.dev, u.width * u.es, u.width * u.es, u.rows, cudaMemcpyDeviceToHost, st);
+  }
+  if (st) {
+    const cudaError_t e2 = cudaStreamSynchronize(st);
+    if (e == cudaSuccess) e = e2;
+  }
+  if (e != cudaSuccess && rc == FRISK_OK) rc = fail_cuda(e, "frisk_b200_quant_run_host");
+  for (Buf& u : b) cudaFree(u.dev);
+  if (st) cudaStreamDestroy(st);
+  if (prev >= 0 && prev != d.device) cudaSetDevice(prev);
+  return rc;
+}
+
+}  // extern "C"

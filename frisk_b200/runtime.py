@@ -80,6 +80,18 @@ class ReduceInfo(C.Structure):
         return {n: int(getattr(self, n)) for n, _ in self._fields_}
 
 
+class QuantDesc(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("ldx", C.c_int64), ("ldo", C.c_int64), ("lds", C.c_int64),
+                ("ldq", C.c_int64), ("kind", C.c_int32), ("in_type", C.c_int32), ("weight_type", C.c_int32),
+                ("q_type", C.c_int32), ("eps", C.c_float), ("device", C.c_int32)]
+
+
+class QuantArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("up", C.c_void_p),
+                ("sum_out", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p), ("stream", C.c_void_p)]
+
+
+QUANT_KINDS = {"plain": 0, "rmsnorm": 1, "silu_mul": 2}
 REDUCE_KINDS = {"add": 0, "mul": 1, "min": 2, "max": 3}
 
 
@@ -189,6 +201,10 @@ def lib() -> C.CDLL:
     L.frisk_b200_reduce_run.restype = C.c_int
     L.frisk_b200_reduce_run_host.argtypes = [C.POINTER(ReduceDesc), vp, vp]
     L.frisk_b200_reduce_run_host.restype = C.c_int
+    L.frisk_b200_quant_run.argtypes = [C.POINTER(QuantDesc), C.POINTER(QuantArgs)]
+    L.frisk_b200_quant_run.restype = C.c_int
+    L.frisk_b200_quant_run_host.argtypes = [C.POINTER(QuantDesc), C.POINTER(QuantArgs)]
+    L.frisk_b200_quant_run_host.restype = C.c_int
     L.frisk_b200_measure_mma_peak.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                               C.POINTER(C.c_double), C.POINTER(C.c_double)]
     L.frisk_b200_measure_mma_peak.restype = C.c_int
@@ -389,6 +405,61 @@ def reduce_host(src: np.ndarray, dst: np.ndarray, dim: int, dtype: int, kind: st
     if dst.size != desc.outer * desc.inner or src.dtype != dst.dtype:
         raise ValueError("destination must have the source's shape without the reduced dimension and its type")
     _check(lib().frisk_b200_reduce_run_host(C.byref(desc), _ptr(src), _ptr(dst)), "reduce_run_host")
+
+
+def quant_desc(rows: int, cols: int, in_type: int, q_type: int, kind: str = "plain", *, eps: float = 1e-6,
+               weight_type: Optional[int] = None, ldx: int = 0, ldo: int = 0, lds: int = 0, ldq: int = 0,
+               device: int = -1) -> QuantDesc:
+    """Rows of 8-bit numbers with scales, made from `rows` x `cols` values: "plain" (the rows of x as they
+    are), "rmsnorm" (after a root-mean-square norm, with the residual added first) or "silu_mul" (of
+    silu(gate) * up).  `ldx`, `ldo` (residual / up), `lds` (sum_out) and `ldq` are row pitches in
+    elements, 0 for packed rows.  See include/frisk_b200.h for the arithmetic."""
+    if kind not in QUANT_KINDS:
+        raise ValueError(f"unsupported quant kind: {kind}. Supported: plain, rmsnorm, silu_mul")
+    return QuantDesc(rows, cols, ldx, ldo, lds, ldq, QUANT_KINDS[kind], in_type,
+                     in_type if weight_type is None else weight_type, q_type, eps, device)
+
+
+def _quant_args(x, q, scale, weight, residual, up, sum_out, stream) -> QuantArgs:
+    return QuantArgs(_ptr(x), _ptr(residual), _ptr(weight), _ptr(up), _ptr(sum_out), _ptr(q), _ptr(scale), stream)
+
+
+def quant_run(desc: QuantDesc, x, q, scale, *, weight=None, residual=None, up=None, sum_out=None,
+              stream: int = 0) -> None:
+    """Asynchronous launch on device buffers (torch CUDA tensors or raw addresses)."""
+    a = _quant_args(x, q, scale, weight, residual, up, sum_out, stream or None)
+    _check(lib().frisk_b200_quant_run(C.byref(desc), C.byref(a)), "quant_run")
+
+
+def quant_host(x: np.ndarray, in_type: int, q_type: int, kind: str = "plain", *, weight: Optional[np.ndarray] = None,
+               weight_type: Optional[int] = None, residual: Optional[np.ndarray] = None, up: Optional[np.ndarray] = None,
+               want_sum: bool = False, eps: float = 1e-6):
+    """Synchronous form on host arrays of raw storage: returns (q, scale), and the sum of x and the
+    residual as a third when `want_sum`."""
+    x = np.ascontiguousarray(x)
+    if x.ndim != 2:
+        raise ValueError("quant_host wants a matrix")
+    halves = kind == "silu_mul" and up is None
+    if halves and x.shape[1] % 2:
+        raise ValueError("gate and up in one matrix need an even number of columns")
+    rows, cols = x.shape[0], x.shape[1] // (2 if halves else 1)
+    desc = quant_desc(rows, cols, in_type, q_type, kind, eps=eps, weight_type=weight_type)
+    other = {}
+    for name, v, shape in (("residual", residual, (rows, cols)), ("up", up, (rows, cols)), ("weight", weight, (cols,))):
+        if v is not None:
+            if tuple(v.shape) != shape:
+                raise ValueError(f"{name} has shape {tuple(v.shape)}, expected {shape}")
+            other[name] = np.ascontiguousarray(v)
+    for name, v, dt in (("x", x, in_type), ("residual", residual, in_type), ("up", up, in_type),
+                        ("weight", weight, desc.weight_type)):
+        if v is not None and v.dtype != W.storage_numpy_dtype(dt):
+            raise ValueError(f"{name} has dtype {v.dtype}, expected {np.dtype(W.storage_numpy_dtype(dt))}")
+    q = np.zeros((rows, cols), W.storage_numpy_dtype(q_type))
+    scale = np.zeros((rows,), np.float32)
+    total = np.zeros((rows, cols), x.dtype) if want_sum else None
+    a = _quant_args(x, q, scale, other.get("weight"), other.get("residual"), other.get("up"), total, None)
+    _check(lib().frisk_b200_quant_run_host(C.byref(desc), C.byref(a)), "quant_run_host")
+    return (q, scale, total) if want_sum else (q, scale)
 
 
 def shard_rows(M: int, nranks: int, rank: int) -> tuple[int, int]:

@@ -6,7 +6,7 @@ distributions of the benchmark configurations (no dataset is involved).  RNG rul
 C order, then round to nearest even into the storage type.
 
 Storage types are carried as numpy arrays of raw bits: float32 -> float32, fp16 -> float16,
-bf16 -> uint16 (upper half of the float32), e4m3fn -> uint8.
+bf16 -> uint16 (upper half of the float32), e4m3fn -> uint8, int8 -> int8.
 """
 from __future__ import annotations
 
@@ -15,9 +15,9 @@ from typing import Optional
 
 import numpy as np
 
-F32, F16, BF16, E4M3, E5M2 = 0, 1, 2, 3, 4  # frisk_dtype of include/frisk_b200.h
-DTYPE_NAMES = {F32: "fp32", F16: "fp16", BF16: "bf16", E4M3: "e4m3fn", E5M2: "e5m2"}
-ELEM_SIZE = {F32: 4, F16: 2, BF16: 2, E4M3: 1, E5M2: 1}
+F32, F16, BF16, E4M3, E5M2, I8 = 0, 1, 2, 3, 4, 5  # frisk_dtype of include/frisk_b200.h
+DTYPE_NAMES = {F32: "fp32", F16: "fp16", BF16: "bf16", E4M3: "e4m3fn", E5M2: "e5m2", I8: "int8"}
+ELEM_SIZE = {F32: 4, F16: 2, BF16: 2, E4M3: 1, E5M2: 1, I8: 1}
 
 
 # --------------------------------------------------------------------------- codecs
@@ -94,6 +94,15 @@ def e5m2_encode(x: np.ndarray) -> np.ndarray:
     return bits | (np.signbit(x).astype(np.uint8) << 7)
 
 
+I8_MAX = 127.0
+QUANT_MAX = {I8: I8_MAX, E4M3: E4M3_MAX, E5M2: E5M2_MAX}  # the largest magnitude of an 8-bit row
+
+
+def i8_encode(x: np.ndarray) -> np.ndarray:
+    """float32 -> int8, round to nearest even, saturating to +-127 (-128 is not used); NaN becomes 0."""
+    return np.nan_to_num(np.clip(np.rint(np.ascontiguousarray(x, dtype=np.float32)), -I8_MAX, I8_MAX), nan=0.0).astype(np.int8)
+
+
 def encode(x: np.ndarray, dtype: int) -> np.ndarray:
     if dtype == F32:
         return np.ascontiguousarray(x, dtype=np.float32)
@@ -105,6 +114,8 @@ def encode(x: np.ndarray, dtype: int) -> np.ndarray:
         return e4m3_encode(x)
     if dtype == E5M2:
         return e5m2_encode(x)
+    if dtype == I8:
+        return i8_encode(x)
     raise ValueError(f"unknown dtype {dtype}")
 
 
@@ -119,11 +130,13 @@ def decode(x: np.ndarray, dtype: int) -> np.ndarray:
         return e4m3_decode(x)
     if dtype == E5M2:
         return e5m2_decode(x)
+    if dtype == I8:
+        return np.asarray(x, dtype=np.int8).astype(np.float32)
     raise ValueError(f"unknown dtype {dtype}")
 
 
 def storage_numpy_dtype(dtype: int):
-    return {F32: np.float32, F16: np.float16, BF16: np.uint16, E4M3: np.uint8, E5M2: np.uint8}[dtype]
+    return {F32: np.float32, F16: np.float16, BF16: np.uint16, E4M3: np.uint8, E5M2: np.uint8, I8: np.int8}[dtype]
 
 
 # --------------------------------------------------------------------------- workloads
@@ -294,6 +307,7 @@ TOLERANCE = {  # (metric, bound) per input type
     BF16: ("max_rel", 1e-2),
     E4M3: ("max_rel", 2e-2),
     E5M2: ("max_rel", 2e-2),
+    I8: ("max_rel", 1e-2),   # the sums are exact: what is left is the rounding into C's type
 }
 
 

@@ -55,9 +55,11 @@ typedef enum {
   FRISK_DT_F16 = 1,
   FRISK_DT_BF16 = 2,
   FRISK_DT_E4M3 = 3, /* "e4m3fn": finite-only fp8, max 448, no inf */
-  FRISK_DT_E5M2 = 4  /* "e5m2": fp8 with fp16's exponent (the top byte of an fp16), max 57344;
+  FRISK_DT_E5M2 = 4, /* "e5m2": fp8 with fp16's exponent (the top byte of an fp16), max 57344;
                         inputs of a gemm only, like e4m3 (the reference names both as buffer
                         element types: ffi/ir.cpp:411-414, 454-457)                      */
+  FRISK_DT_I8 = 5    /* signed 8-bit integers: inputs of a gemm and outputs of
+                        frisk_b200_quant_run only                                        */
 } frisk_dtype;
 
 typedef enum { FRISK_SCALE_NONE = 0, FRISK_SCALE_ROW_COL = 1 } frisk_scale_mode;
@@ -341,6 +343,67 @@ int frisk_b200_reduce_run(const frisk_reduce_desc* desc, const void* src, void* 
                           size_t ws_bytes, void* stream);
 /* The same on HOST buffers: allocates, copies in, runs, copies dst back, synchronises. */
 int frisk_b200_reduce_run_host(const frisk_reduce_desc* desc, const void* src, void* dst);
+
+/* ---- rows of 8-bit numbers with scales --------------------------------------------------- */
+/*
+ * Makes the operands of an 8-bit gemm on the device: rows of i8, e4m3 or e5m2 numbers with one fp32
+ * scale each, in the order a K-innermost operand is stored (A by tokens, B by output channels), so
+ * that q goes in as A or B and the scales as scale_a or scale_b.
+ *   FRISK_QUANT_PLAIN     v = x
+ *   FRISK_QUANT_RMSNORM   h = x + residual (no residual: h = x),
+ *                         v = h * rsqrt(mean over the row of h^2 + eps) * weight (NULL: ones);
+ *                         sum_out (may be NULL) = h rounded to the input type
+ *   FRISK_QUANT_SILU_MUL  v = gate / (1 + exp(-gate)) * up, with x = gate and `up` the other matrix;
+ *                         `up` NULL: x holds rows of 2 * cols elements, the gate and then the up half
+ *   scale[r] = max(max |v[r, :]| / Q, 2^-126),  q[r, c] = nearest-even(v[r, c] / scale[r])
+ * with Q = 127 (i8: -128 is not used), 448 (e4m3), 57344 (e5m2).  Arithmetic in fp32 (the norm is of
+ * the unrounded h; squares are summed in fp32, so the rows' norms have to stay below 1e19), one
+ * rounding into q and one into sum_out.  A row with an infinity or NaN in v, or with squares that
+ * overflow, gets a scale of infinity or NaN; its q are 0 or NaN (i8 has no NaN: 0), and every product
+ * with its scale is NaN.  A row of zeros gets q = 0 and the scale 2^-126.  The order of the sum is
+ * fixed by the shape, the types and the alignment.
+ */
+typedef enum {
+  FRISK_QUANT_PLAIN = 0,
+  FRISK_QUANT_RMSNORM = 1,
+  FRISK_QUANT_SILU_MUL = 2
+} frisk_quant_kind;
+
+typedef struct frisk_quant_desc {
+  int64_t rows, cols;      /* of q; cols >= 1, no rows: nothing is done                          */
+  int64_t ldx;             /* row pitches in ELEMENTS, 0 = packed: x,                            */
+  int64_t ldo;             /* the residual or the up matrix,                                     */
+  int64_t lds;             /* sum_out,                                                           */
+  int64_t ldq;             /* q                                                                  */
+  int32_t kind;            /* frisk_quant_kind                                                   */
+  int32_t in_type;         /* FRISK_DT_F32, _F16 or _BF16: x, residual, up, sum_out              */
+  int32_t weight_type;     /* rmsnorm: in_type or FRISK_DT_F32                                   */
+  int32_t q_type;          /* FRISK_DT_I8, _E4M3 or _E5M2                                        */
+  float eps;               /* rmsnorm; >= 0                                                      */
+  int32_t device;          /* CUDA ordinal, -1 = current                                         */
+} frisk_quant_desc;
+
+typedef struct frisk_quant_args {
+  const void* x;
+  const void* residual;    /* rmsnorm; may be NULL                                               */
+  const void* weight;      /* rmsnorm, [cols]; may be NULL                                       */
+  const void* up;          /* silu_mul; may be NULL                                              */
+  void* sum_out;           /* rmsnorm with a residual; may be NULL, x or the residual            */
+  void* q;
+  float* scale;            /* [rows]                                                             */
+  void* stream;
+} frisk_quant_args;
+
+/*
+ * Stream-ordered, asynchronous, one launch, no workspace.  Device pointers aligned to their element
+ * size (16-byte alignment of rows enables vector loads; any width and pitch is accepted).  q, scale
+ * and sum_out must not overlap anything else, but for sum_out in place of x or of the residual (the
+ * same pointer and pitch).
+ */
+int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* args);
+/* The same on HOST buffers (args->stream is not used): allocates, copies in, runs, copies q, scale
+ * and sum_out back, synchronises. */
+int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_args* args);
 
 /* ---- layout mapping ------------------------------------------------------------------- */
 /*

@@ -152,3 +152,46 @@ def ref_reduce(src: np.ndarray, dim: int, dtype: int, kind: str, clear: bool = T
         out = fold(d0, out)
         mag = mag + np.abs(d0) if kind == "add" else np.abs(out)
     return out, mag
+
+
+def round8(v: np.ndarray, q_type: int) -> np.ndarray:
+    """float64 -> the nearest number of an 8-bit type, ties to even, saturating, in float64 (no
+    detour over float32, whose own rounding would move values onto ties).  NaN stays NaN."""
+    v = np.asarray(v, dtype=np.float64)
+    top = W.QUANT_MAX[q_type]
+    if q_type == W.I8:
+        return np.clip(np.rint(v), -top, top)
+    mantissa, least = (3, -6) if q_type == W.E4M3 else (2, -14)
+    with np.errstate(invalid="ignore"):
+        exponent = np.maximum(np.frexp(np.abs(v))[1] - 1, least)
+        step = np.ldexp(1.0, exponent - mantissa)
+        return np.clip(np.rint(v / step) * step, -top, top)
+
+
+def ref_quant(x: np.ndarray, in_type: int, kind: str, *, weight: Optional[np.ndarray] = None,
+              weight_type: Optional[int] = None, residual: Optional[np.ndarray] = None,
+              up: Optional[np.ndarray] = None, eps: float = 1e-6) -> tuple[np.ndarray, Optional[np.ndarray]]:
+    """The values that frisk_b200_quant_run turns into 8-bit rows, in float64 from the exactly decoded
+    inputs (raw storage): (v, h) with h = x + residual for "rmsnorm", None otherwise.  The 8-bit rows
+    themselves follow from v by ``quant_scale`` and ``round8``."""
+    f = lambda a, t: W.decode(np.asarray(a), t).astype(np.float64)  # noqa: E731
+    v = f(x, in_type)
+    if kind == "plain":
+        return v, None
+    with np.errstate(all="ignore"):
+        if kind == "silu_mul":
+            if up is None:
+                gate, u = np.split(v, 2, axis=1)
+            else:
+                gate, u = v, f(up, in_type)
+            return gate / (1.0 + np.exp(-gate)) * u, None
+        h = v if residual is None else v + f(residual, in_type)
+        n = h / np.sqrt(np.mean(h * h, axis=1, keepdims=True) + np.float64(np.float32(eps)))
+        if weight is not None:
+            n = n * f(weight, in_type if weight_type is None else weight_type)
+        return n, h
+
+
+def quant_scale(v: np.ndarray, q_type: int) -> np.ndarray:
+    """The scale of every row of v (float64): its largest magnitude over the type's, at least 2^-126."""
+    return np.maximum(np.abs(v).max(axis=1) / W.QUANT_MAX[q_type], 2.0 ** -126)
