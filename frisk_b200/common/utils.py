@@ -15,7 +15,7 @@ __all__ = ["create_context", "create_session", "FriskHelper"]
 
 _TYPE_GETTERS = {
     "fp16": "get_f16_ty", "bf16": "get_bf16_ty", "fp32": "get_f32_ty", "fp64": "get_f64_ty",
-    "int64": "get_int64_ty", "e4m3fn": "get_f8e4m3fn_ty", "e5m2": "get_f8e5m2_ty",
+    "int8": "get_int8_ty", "int64": "get_int64_ty", "e4m3fn": "get_f8e4m3fn_ty", "e5m2": "get_f8e5m2_ty",
 }
 
 

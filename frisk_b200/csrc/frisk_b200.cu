@@ -47,10 +47,15 @@ int elem_size(int dt) {
     case FRISK_DT_BF16: return 2;
     case FRISK_DT_E4M3: return 1;
     case FRISK_DT_E5M2: return 1;
+    case FRISK_DT_I8: return 1;
     default: return 0;
   }
 }
 bool is_fp8(int dt) { return dt == FRISK_DT_E4M3 || dt == FRISK_DT_E5M2; }
+bool is_8bit(int dt) { return is_fp8(dt) || dt == FRISK_DT_I8; }
+// The longest K of an integer product: 131071 * 2^14 is the largest sum of products of two 8-bit
+// integers that 32 bits hold.
+constexpr int64_t kMaxIntK = (1ll << 17) - 1;
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -977,6 +982,7 @@ int launch_simt(const frisk_gemm_desc& d, const void* A, const void* B, void* C,
     case FRISK_DT_BF16: return launch_simt_in<__nv_bfloat16>(d, sp, st);
     case FRISK_DT_E4M3: return launch_simt_in<frisk::e4m3_t>(d, sp, st);
     case FRISK_DT_E5M2: return launch_simt_in<frisk::e5m2_t>(d, sp, st);
+    case FRISK_DT_I8: return launch_simt_in<int8_t>(d, sp, st);
     default: return FRISK_ERR_UNSUPPORTED;
   }
 }
@@ -1030,7 +1036,11 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
   if (d.M <= 0 || d.N <= 0 || d.K <= 0) return FRISK_ERR_INVALID_ARGUMENT;
   if (!elem_size(d.a_type) || !elem_size(d.b_type) || !elem_size(d.c_type))
     return FRISK_ERR_INVALID_ARGUMENT;
-  if (is_fp8(d.c_type)) return FRISK_ERR_UNSUPPORTED;
+  if (is_8bit(d.c_type)) return FRISK_ERR_UNSUPPORTED;
+  if (d.a_type == FRISK_DT_I8 && d.K > kMaxIntK) {
+    g_last_error = "an integer product of more than 131071 terms could overflow 32 bits";
+    return FRISK_ERR_TOO_LARGE;
+  }
   if (d.a_type != d.b_type) return FRISK_ERR_INVALID_ARGUMENT;  // ffi/ir.cpp:357-359
   if (d.scale_mode != FRISK_SCALE_NONE && d.scale_mode != FRISK_SCALE_ROW_COL)
     return FRISK_ERR_INVALID_ARGUMENT;
@@ -1794,7 +1804,7 @@ int frisk_b200_gemm_skinny_static(const frisk_gemm_desc* desc, const void* A, co
   frisk_gemm_desc d = *desc;
   if (d.M <= 0 || d.N <= 0 || d.K <= 0) return FRISK_ERR_INVALID_ARGUMENT;
   if (!elem_size(d.a_type) || d.a_type != d.b_type || !elem_size(d.c_type) ||
-      is_fp8(d.c_type))
+      is_8bit(d.c_type))
     return FRISK_ERR_INVALID_ARGUMENT;
   if (d.scale_mode != FRISK_SCALE_NONE && d.scale_mode != FRISK_SCALE_ROW_COL)
     return FRISK_ERR_INVALID_ARGUMENT;
@@ -1892,7 +1902,7 @@ size_t frisk_b200_gemm_skinny_static_capacity(void) { return kStaticScratchFloat
 int frisk_b200_measure_mma_peak(int32_t ab_type, int32_t pair, int32_t k_blocks, int32_t reps,
                                 double* tflops, double* ms_per_launch) {
   if (!tflops || k_blocks < 32 || k_blocks % 32 || reps < 1) return FRISK_ERR_INVALID_ARGUMENT;
-  if (!elem_size(ab_type)) return FRISK_ERR_UNSUPPORTED;   // fp32 is measured as kind::tf32
+  if (!elem_size(ab_type) || ab_type == FRISK_DT_I8) return FRISK_ERR_UNSUPPORTED;   // fp32 is measured as kind::tf32
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();

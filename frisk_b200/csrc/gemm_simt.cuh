@@ -40,6 +40,20 @@ __device__ __forceinline__ float cast_in<e5m2_t>(e5m2_t v) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(v.bits, __NV_E5M2)));
 }
 
+// What an input type is multiplied and summed in: fp32, or 32-bit integers for 8-bit integers (exact).
+template <typename TIn>
+struct SimtAcc {
+  using type = float;
+  static __device__ __forceinline__ float load(TIn v) { return cast_in<TIn>(v); }
+  static __device__ __forceinline__ float mac(float a, float b, float c) { return fmaf(a, b, c); }
+};
+template <>
+struct SimtAcc<int8_t> {
+  using type = int;
+  static __device__ __forceinline__ int load(int8_t v) { return v; }
+  static __device__ __forceinline__ int mac(int a, int b, int c) { return a * b + c; }
+};
+
 constexpr int kSimtTile = 64;
 constexpr int kSimtBK = 16;
 
@@ -50,10 +64,11 @@ template <typename TIn, typename TOut, int TM>
 __global__ void __launch_bounds__(TM * 4)
 gemm_simt_kernel(const SimtParams p) {
   constexpr int kThreads = TM * 4;
+  using Acc = typename SimtAcc<TIn>::type;
   // rows are 16-byte multiples apart and every thread reads its four values at a 16-byte offset,
   // so the inner loop reads each operand with one 128-bit load
-  __shared__ __align__(16) float As[kSimtBK][TM + 4];         // [k][m]
-  __shared__ __align__(16) float Bs[kSimtBK][kSimtTile + 4];  // [k][n]
+  __shared__ __align__(16) Acc As[kSimtBK][TM + 4];         // [k][m]
+  __shared__ __align__(16) Acc Bs[kSimtBK][kSimtTile + 4];  // [k][n]
   const TIn* A = reinterpret_cast<const TIn*>(p.A);
   const TIn* B = reinterpret_cast<const TIn*>(p.B);
   TOut* C = reinterpret_cast<TOut*>(p.C);
@@ -62,17 +77,17 @@ gemm_simt_kernel(const SimtParams p) {
   const int tx = threadIdx.x & 15;  // column group
   const int ty = threadIdx.x >> 4;  // row group
 
-  float acc[4][4];
+  Acc acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[i][j] = Acc(0);
 
   // The K slice after the one being multiplied is fetched into registers while the FMAs run, so
   // the global-memory latency of a slice is paid once, not once per slice.
   constexpr int kAPer = TM * kSimtBK / kThreads;         // 4 elements of the A slice per thread
   constexpr int kBPer = kSimtTile * kSimtBK / kThreads;  // 4 or 8 of the B slice
-  float av[kAPer], bv[kBPer];
+  Acc av[kAPer], bv[kBPer];
   // walk the contiguous global dimension with consecutive threads
   auto a_pos = [&](int idx, int& am, int& ak) {
     if (p.transA) { am = idx & (TM - 1); ak = idx / TM; } else { ak = idx & 15; am = idx >> 4; }
@@ -85,20 +100,20 @@ gemm_simt_kernel(const SimtParams p) {
     for (int e = 0; e < kAPer; ++e) {
       int am, ak;
       a_pos(threadIdx.x + e * kThreads, am, ak);
-      av[e] = 0.f;
+      av[e] = Acc(0);
       if (m0 + am < p.M && k0 + ak < p.K) {
         const int64_t off = p.transA ? (k0 + ak) * p.lda + (m0 + am) : (m0 + am) * p.lda + (k0 + ak);
-        av[e] = cast_in<TIn>(A[off]);
+        av[e] = SimtAcc<TIn>::load(A[off]);
       }
     }
 #pragma unroll
     for (int e = 0; e < kBPer; ++e) {
       int bn, bk;
       b_pos(threadIdx.x + e * kThreads, bn, bk);
-      bv[e] = 0.f;
+      bv[e] = Acc(0);
       if (n0 + bn < p.N && k0 + bk < p.K) {
         const int64_t off = p.transB ? (n0 + bn) * p.ldb + (k0 + bk) : (k0 + bk) * p.ldb + (n0 + bn);
-        bv[e] = cast_in<TIn>(B[off]);
+        bv[e] = SimtAcc<TIn>::load(B[off]);
       }
     }
   };
@@ -120,13 +135,15 @@ gemm_simt_kernel(const SimtParams p) {
     if (k0 + kSimtBK < p.K) fetch(k0 + kSimtBK);
 #pragma unroll
     for (int kk = 0; kk < kSimtBK; ++kk) {
-      const float4 a4 = *reinterpret_cast<const float4*>(&As[kk][ty * 4]);
-      const float4 b4 = *reinterpret_cast<const float4*>(&Bs[kk][tx * 4]);
-      const float a[4] = {a4.x, a4.y, a4.z, a4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+      struct alignas(16) Four {
+        Acc v[4];
+      };
+      const Four a = *reinterpret_cast<const Four*>(&As[kk][ty * 4]);
+      const Four b = *reinterpret_cast<const Four*>(&Bs[kk][tx * 4]);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = SimtAcc<TIn>::mac(a.v[i], b.v[j], acc[i][j]);
     }
     __syncthreads();
   }
@@ -140,7 +157,7 @@ gemm_simt_kernel(const SimtParams p) {
     for (int j = 0; j < 4; ++j) {
       const int64_t n = n0 + tx * 4 + j;
       if (n >= p.N) continue;
-      float v = acc[i][j] * sa;
+      float v = (float)acc[i][j] * sa;
       if (p.scale_b) v *= p.scale_b[n];
       TOut* dst = C + m * p.ldc + n;
       if (!p.clear_accum) v += cast_in<TOut>(*dst);

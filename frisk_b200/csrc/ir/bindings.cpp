@@ -756,6 +756,7 @@ void initBuilder(py::module_& m) {
       .def("get_int64_tensor", [tensorConstant](PyBuilder& s, std::vector<double> v, std::vector<int64_t> sh) { return tensorConstant(s, v, sh, makeScalar(TypeKind::Integer, 64), true); })
       // types
       .def("get_bool_ty", [](PyBuilder&) { return castType(makeScalar(TypeKind::Integer, 8)); })
+      .def("get_int8_ty", [](PyBuilder&) { return castType(makeScalar(TypeKind::Integer, 8)); })            // addition
       .def("get_int64_ty", [](PyBuilder&) { return castType(makeScalar(TypeKind::Integer, 64)); })
       .def("get_index_ty", [](PyBuilder&) { return castType(makeScalar(TypeKind::Index)); })  // addition
       .def("get_f64_ty", [](PyBuilder&) { return castType(makeScalar(TypeKind::F64)); })
@@ -847,17 +848,17 @@ void initBuilder(py::module_& m) {
         const int64_t n = need(b->shape[1], "N dimension of B");
         if (mm != need(c->shape[0], "M dimension of C") || n != need(c->shape[1], "N dimension of C"))
           throw std::invalid_argument("create_gemm_op expects C shape to match A/B product");
-        const bool fp8 = a->element->kind == TypeKind::F8E4M3FN || a->element->kind == TypeKind::F8E5M2;
-        // the reference requires one element type for all three (ffi/ir.cpp:357-359); 8-bit float
-        // inputs, which it cannot express at all, may pair with a wider C
-        if (!typeEqual(a->element, b->element) || (!typeEqual(a->element, c->element) && !fp8))
+        const bool narrow = isNarrowGemmInput(a->element);
+        // the reference requires one element type for all three (ffi/ir.cpp:357-359); 8-bit
+        // inputs, whose product it cannot express at all, may pair with a wider C
+        if (!typeEqual(a->element, b->element) || (!typeEqual(a->element, c->element) && !narrow))
           throw std::invalid_argument("create_gemm_op expects operands to have matching element types");
         // addition: per-row scales of A and per-column scales of B (fp32 vectors of M and N
-        // entries) for 8-bit float inputs; the reference's op has three operands only
+        // entries) for 8-bit inputs; the reference's op has three operands only
         if (scaleA.has_value() != scaleB.has_value())
           throw std::invalid_argument("create_gemm_op expects scale_a and scale_b together");
         if (scaleA) {
-          if (!fp8) throw std::invalid_argument("create_gemm_op takes scales only with 8-bit float operands");
+          if (!narrow) throw std::invalid_argument("create_gemm_op takes scales only with 8-bit float or integer operands");
           auto vec = [](Value v, int64_t n, const char* what) {
             const TypeStorage* t = requireMemRef(v, what);
             if (t->shape.size() != 1 || t->shape[0] != n || t->element->kind != TypeKind::F32)

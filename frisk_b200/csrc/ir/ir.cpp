@@ -59,6 +59,9 @@ bool typeEqual(const Type& a, const Type& b) {
     default: return true;
   }
 }
+bool isNarrowGemmInput(const Type& t) {
+  return t && (t->kind == TypeKind::F8E4M3FN || t->kind == TypeKind::F8E5M2 || (t->kind == TypeKind::Integer && t->width == 8));
+}
 bool isFloat(const Type& t) { return t && t->kind <= TypeKind::F8E5M2; }
 unsigned bitWidth(const Type& t) {
   switch (t->kind) {
@@ -599,9 +602,9 @@ static std::string verifyOne(Operation* op) {
     auto *A = memref(op->operands[0]), *B = memref(op->operands[1]), *C = memref(op->operands[2]);
     if (!A || !B || !C) return "operands must be memrefs";
     const bool sameAB = typeEqual(A->element, B->element);
-    const bool fp8 = A->element->kind == TypeKind::F8E4M3FN || A->element->kind == TypeKind::F8E5M2;
-    // extension: 8-bit float inputs may produce a wider C (the reference has no fp8 GEMM)
-    if (!sameAB || (!typeEqual(A->element, C->element) && !fp8))
+    const bool narrow = isNarrowGemmInput(A->element);
+    // extension: 8-bit inputs may produce a wider C (the reference has no 8-bit GEMM)
+    if (!sameAB || (!typeEqual(A->element, C->element) && !narrow))
       return "all operands must have the same element type";
     if (A->shape[1] != B->shape[0]) return "A columns must equal B rows for matrix multiplication";
     if (A->shape[0] != C->shape[0] || B->shape[1] != C->shape[1])

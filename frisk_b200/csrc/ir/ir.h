@@ -89,6 +89,7 @@ Type makeFunction(std::vector<Type> in, std::vector<Type> out);
 bool typeEqual(const Type& a, const Type& b);
 std::string printType(const Type& t);
 bool isFloat(const Type& t);
+bool isNarrowGemmInput(const Type& t);  // 8-bit floats and integers: inputs of a gemm with a wider result
 unsigned bitWidth(const Type& t);
 
 // ---------------------------------------------------------------------------- attributes

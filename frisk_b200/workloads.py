@@ -15,7 +15,7 @@ from typing import Optional
 
 import numpy as np
 
-F32, F16, BF16, E4M3, E5M2, I8 = 0, 1, 2, 3, 4, 5  # frisk_dtype of include/frisk_b200.h
+F32, F16, BF16, E4M3, E5M2, I8 = 0, 1, 2, 3, 4, 6  # frisk_dtype of include/frisk_b200.h
 DTYPE_NAMES = {F32: "fp32", F16: "fp16", BF16: "bf16", E4M3: "e4m3fn", E5M2: "e5m2", I8: "int8"}
 ELEM_SIZE = {F32: 4, F16: 2, BF16: 2, E4M3: 1, E5M2: 1, I8: 1}
 

@@ -23,6 +23,9 @@
  * Semantics (include/Dialect/Frisk/IR/FriskOps.td:248-289):
  *   C = (clear_accum ? 0 : C) + scale_a[m] * scale_b[n] * sum_k A[m,k] * B[k,n]
  * with the products and the sum in fp32 and one round-to-nearest-even cast to C's type.
+ * FRISK_DT_I8 operands: the sum is exact, in 32-bit integers (K up to 131071, so that it cannot
+ * overflow), converted to fp32 once, scaled by scale_a and scale_b (two fp32 products) and rounded
+ * into C.
  * The scales are an addition to the reference op (it has no fp8 GEMM); they are optional.
  */
 #ifndef FRISK_B200_H_
@@ -58,8 +61,8 @@ typedef enum {
   FRISK_DT_E5M2 = 4, /* "e5m2": fp8 with fp16's exponent (the top byte of an fp16), max 57344;
                         inputs of a gemm only, like e4m3 (the reference names both as buffer
                         element types: ffi/ir.cpp:411-414, 454-457)                      */
-  FRISK_DT_I8 = 5    /* signed 8-bit integers: inputs of a gemm and outputs of
-                        frisk_b200_quant_run only                                        */
+  FRISK_DT_I8 = 6    /* signed 8-bit integers: inputs of a gemm and outputs of
+                        frisk_b200_quant_run only (5 is no type)                         */
 } frisk_dtype;
 
 typedef enum { FRISK_SCALE_NONE = 0, FRISK_SCALE_ROW_COL = 1 } frisk_scale_mode;

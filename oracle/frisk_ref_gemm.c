@@ -27,7 +27,7 @@
 #include <omp.h>
 #endif
 
-enum { REF_F32 = 0, REF_F16 = 1, REF_BF16 = 2, REF_E4M3 = 3, REF_E5M2 = 4 };
+enum { REF_F32 = 0, REF_F16 = 1, REF_BF16 = 2, REF_E4M3 = 3, REF_E5M2 = 4, REF_I8 = 6 };
 
 typedef struct frisk_ref_desc {
   int64_t M, N, K;
@@ -118,6 +118,7 @@ static float decode_in(const void* p, int64_t i, int type) {
     case REF_F16: return frisk_ref_decode_f16(((const uint16_t*)p)[i]);
     case REF_BF16: return frisk_ref_decode_bf16(((const uint16_t*)p)[i]);
     case REF_E4M3: return frisk_ref_decode_e4m3(((const uint8_t*)p)[i]);
+    case REF_I8: return (float)((const int8_t*)p)[i];
     default: return frisk_ref_decode_e5m2(((const uint8_t*)p)[i]);
   }
 }
@@ -132,7 +133,7 @@ static void store_out(void* p, int64_t i, int type, float v) {
 
 static int valid_desc(const frisk_ref_desc* d) {
   if (!d || d->M <= 0 || d->N <= 0 || d->K <= 0) return 0;
-  if (d->ab_type < 0 || d->ab_type > 4 || d->c_type < 0 || d->c_type > 2) return 0;
+  if (d->ab_type < 0 || (d->ab_type > 4 && d->ab_type != REF_I8) || d->c_type < 0 || d->c_type > 2) return 0;
   if (d->lda < (d->transA ? d->M : d->K)) return 0;
   if (d->ldb < (d->transB ? d->K : d->N)) return 0;
   if (d->ldc < d->N) return 0;
