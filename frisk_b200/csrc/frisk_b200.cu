@@ -186,11 +186,12 @@ int fill_operand(frisk::OperandParams& o, frisk_tma_params& lay, bool mn_major, 
 }
 
 uint32_t make_idesc(int ab_type, bool a_mn_major, bool b_mn_major, uint32_t m, uint32_t n) {
-  uint32_t fmt = 0;  // kind::f16: 0 = f16, 1 = bf16; kind::f8f6f4: 0 = e4m3, 1 = e5m2; kind::tf32: 2 = tf32
-  if (ab_type == FRISK_DT_BF16 || ab_type == FRISK_DT_E5M2) fmt = 1;
+  // kind::f16: 0 = f16, 1 = bf16; kind::f8f6f4: 0 = e4m3, 1 = e5m2; kind::tf32: 2 = tf32; kind::i8: 1 = signed
+  uint32_t fmt = 0;
+  if (ab_type == FRISK_DT_BF16 || ab_type == FRISK_DT_E5M2 || ab_type == FRISK_DT_I8) fmt = 1;
   if (ab_type == FRISK_DT_F32) fmt = 2;
   uint32_t d = 0;
-  d |= 1u << 4;  // fp32 accumulator
+  d |= (ab_type == FRISK_DT_I8 ? 2u : 1u) << 4;  // 32-bit integer / fp32 accumulator
   d |= fmt << 7;
   d |= fmt << 10;
   d |= (a_mn_major ? 1u : 0u) << 15;
@@ -289,13 +290,13 @@ constexpr size_t kLaunchDynSmem = kMaxDynSmem;
 
 // Why a problem cannot take the tensor-core kernels (FRISK_TC_*; 0 = it can).
 int tcgen05_ineligible_reason(const frisk_gemm_desc& d) {
-  if (d.a_type != FRISK_DT_F16 && d.a_type != FRISK_DT_BF16 && !is_fp8(d.a_type))
+  if (d.a_type != FRISK_DT_F16 && d.a_type != FRISK_DT_BF16 && !is_8bit(d.a_type))
     return FRISK_TC_INPUT_TYPE;
   const int es = elem_size(d.a_type);
   if ((d.lda * es) % 16 || (d.ldb * es) % 16) return FRISK_TC_PITCH;
   if (d.M >= (1ll << 31) || d.N >= (1ll << 31) || d.K >= (1ll << 31)) return FRISK_TC_EXTENT;
   // 8-bit operands are taken K-major only (A row-major, B column-major)
-  if (is_fp8(d.a_type) && (d.transA || !d.transB)) return FRISK_TC_FP8_ORDER;
+  if (is_8bit(d.a_type) && (d.transA || !d.transB)) return FRISK_TC_FP8_ORDER;
   return FRISK_TC_OK;
 }
 bool tcgen05_eligible(const frisk_gemm_desc& d) { return tcgen05_ineligible_reason(d) == FRISK_TC_OK; }
@@ -650,13 +651,13 @@ int ensure_dyn_smem(Kern kern, int device) {
   if (tracked) __atomic_store_n(&done[device], true, __ATOMIC_RELEASE);
   return FRISK_OK;
 }
-template <typename TC, bool kSplit, bool kTf32 = false> struct OneCtaKernelTag {};
-template <typename TC, bool kTf32 = false> struct PairKernelTag {};
+template <typename TC, bool kSplit, bool kTf32 = false, bool kInt = false> struct OneCtaKernelTag {};
+template <typename TC, bool kTf32 = false, bool kInt = false> struct PairKernelTag {};
 
-template <typename TC, bool kSplit, bool kTf32 = false>
+template <typename TC, bool kSplit, bool kTf32 = false, bool kInt = false>
 int launch_tcgen05_ts(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
-  auto kern = frisk::gemm_tcgen05_kernel<TC, kSplit, kTf32>;
-  if (int rc = ensure_dyn_smem<OneCtaKernelTag<TC, kSplit, kTf32>>(kern, pl->device)) return rc;
+  auto kern = frisk::gemm_tcgen05_kernel<TC, kSplit, kTf32, kInt>;
+  if (int rc = ensure_dyn_smem<OneCtaKernelTag<TC, kSplit, kTf32, kInt>>(kern, pl->device)) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)pl->info.num_ctas, 1, 1);
@@ -682,10 +683,10 @@ int launch_tcgen05_ts(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStrea
 }
 
 // How many clusters of the plan's size the device can hold at once, for one C type.
-template <typename TC>
-int max_active_clusters_t(frisk_gemm_plan* pl, int* out) {
-  auto kern = frisk::gemm_tcgen05_kernel<TC, true>;
-  if (int rc = ensure_dyn_smem<OneCtaKernelTag<TC, true>>(kern, pl->device)) return rc;
+template <typename TC, bool kInt>
+int max_active_clusters_ti(frisk_gemm_plan* pl, int* out) {
+  auto kern = frisk::gemm_tcgen05_kernel<TC, true, false, kInt>;
+  if (int rc = ensure_dyn_smem<OneCtaKernelTag<TC, true, false, kInt>>(kern, pl->device)) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)pl->info.num_ctas, 1, 1);
@@ -700,6 +701,11 @@ int max_active_clusters_t(frisk_gemm_plan* pl, int* out) {
   cfg.numAttrs = 1;
   FRISK_CUDA(cudaOccupancyMaxActiveClusters(out, kern, &cfg));
   return FRISK_OK;
+}
+
+template <typename TC>
+int max_active_clusters_t(frisk_gemm_plan* pl, int* out) {
+  return pl->d.a_type == FRISK_DT_I8 ? max_active_clusters_ti<TC, true>(pl, out) : max_active_clusters_ti<TC, false>(pl, out);
 }
 
 bool skinny_clusters_fit(frisk_gemm_plan* pl) {
@@ -719,13 +725,16 @@ bool skinny_clusters_fit(frisk_gemm_plan* pl) {
 
 template <typename TC>
 int launch_tcgen05_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
+  if (pl->d.a_type == FRISK_DT_I8)
+    return g.split_mode ? launch_tcgen05_ts<TC, true, false, true>(pl, g, st)
+                        : launch_tcgen05_ts<TC, false, false, true>(pl, g, st);
   return g.split_mode ? launch_tcgen05_ts<TC, true>(pl, g, st) : launch_tcgen05_ts<TC, false>(pl, g, st);
 }
 
-template <typename TC, bool kTf32 = false>
+template <typename TC, bool kTf32 = false, bool kInt = false>
 int launch_pair_tf(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
-  auto kern = frisk::gemm_tcgen05_pair_kernel<TC, kTf32>;
-  if (int rc = ensure_dyn_smem<PairKernelTag<TC, kTf32>>(kern, pl->device)) return rc;
+  auto kern = frisk::gemm_tcgen05_pair_kernel<TC, kTf32, kInt>;
+  if (int rc = ensure_dyn_smem<PairKernelTag<TC, kTf32, kInt>>(kern, pl->device)) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)pl->info.num_ctas, 1, 1);
@@ -747,17 +756,16 @@ int launch_pair_tf(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t
 
 template <typename TC>
 int launch_pair_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
-  return launch_pair_tf<TC>(pl, g, st);
+  return pl->d.a_type == FRISK_DT_I8 ? launch_pair_tf<TC, false, true>(pl, g, st) : launch_pair_tf<TC>(pl, g, st);
 }
 
 // The CTA-pair kernel with K split over the pairs of a cluster: one cluster of 2 x cluster_k CTAs
 // per tile.  `occupancy`: ask how many such clusters the device holds at once instead of launching.
-template <typename TC> struct PairKsplitKernelTag {};
-template <typename TC>
-int launch_pair_ksplit_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st,
-                         int* occupancy = nullptr) {
-  auto kern = frisk::gemm_tcgen05_pair_ksplit_kernel<TC>;
-  if (int rc = ensure_dyn_smem<PairKsplitKernelTag<TC>>(kern, pl->device)) return rc;
+template <typename TC, bool kInt> struct PairKsplitKernelTag {};
+template <typename TC, bool kInt>
+int launch_pair_ksplit_ti(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st, int* occupancy) {
+  auto kern = frisk::gemm_tcgen05_pair_ksplit_kernel<TC, kInt>;
+  if (int rc = ensure_dyn_smem<PairKsplitKernelTag<TC, kInt>>(kern, pl->device)) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)pl->info.num_ctas, 1, 1);
@@ -780,6 +788,12 @@ int launch_pair_ksplit_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaSt
   cfg.numAttrs = 2;
   FRISK_CUDA(cudaLaunchKernelEx(&cfg, kern, pl->tmap_a, pl->tmap_b, g));
   return FRISK_OK;
+}
+
+template <typename TC>
+int launch_pair_ksplit_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st, int* occupancy) {
+  return pl->d.a_type == FRISK_DT_I8 ? launch_pair_ksplit_ti<TC, true>(pl, g, st, occupancy)
+                                     : launch_pair_ksplit_ti<TC, false>(pl, g, st, occupancy);
 }
 
 int launch_pair_ksplit(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st, int* occupancy = nullptr) {
@@ -838,7 +852,8 @@ int launch_kplanes_sum_t(const frisk_gemm_plan* pl, const frisk::GemmParams& g, 
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   const int vec_ok = ((uintptr_t)C % (4 * sizeof(TC)) == 0) && (d.ldc % 4 == 0);
-  FRISK_CUDA(cudaLaunchKernelEx(&cfg, frisk::kplanes_sum_kernel<TC>, planes, (uint64_t)g.plane_elems,
+  auto kern = d.a_type == FRISK_DT_I8 ? frisk::kplanes_sum_kernel<TC, true> : frisk::kplanes_sum_kernel<TC, false>;
+  FRISK_CUDA(cudaLaunchKernelEx(&cfg, kern, planes, (uint64_t)g.plane_elems,
                                 (uint32_t)g.k_parts, (int64_t)g.ldc, reinterpret_cast<TC*>(C), (int64_t)d.ldc,
                                 (int64_t)d.M, (int64_t)d.N, sa, sb, (int)(d.clear_accum ? 1 : 0), vec_ok));
   return FRISK_OK;
@@ -1535,7 +1550,8 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
   if (pl->pair_cluster) {
     rc = launch_pair_ksplit(pl, g, st);
   } else if (planes) {
-    rc = launch_pair_t<float>(pl, g, st);
+    // (an integer product's planes are its raw 32-bit sums)
+    rc = d.a_type == FRISK_DT_I8 ? launch_pair_tf<int32_t, false, true>(pl, g, st) : launch_pair_t<float>(pl, g, st);
     if (!rc) {
       const float* w = static_cast<const float*>(workspace);
       switch (d.c_type) {
@@ -1829,6 +1845,8 @@ int frisk_b200_gemm_skinny_static(const frisk_gemm_desc* desc, const void* A, co
   d.force_kernel = 0;
   d.tile_n = 0;
   d.band_tiles = 0;
+  // the scratch holds fp32 partial sums, which would lose the exactness of an integer product
+  if (d.a_type == FRISK_DT_I8) return FRISK_ERR_UNSUPPORTED;
   // only the few-row plan uses scratch; everything else has no reason to come through here
   // (this entry point keeps the 64-row limit the few-row plan had when it was written)
   if (!(tcgen05_eligible(d) && d.M <= 64 && skinny_shape(d, 1024))) return FRISK_ERR_UNSUPPORTED;
@@ -1902,7 +1920,7 @@ size_t frisk_b200_gemm_skinny_static_capacity(void) { return kStaticScratchFloat
 int frisk_b200_measure_mma_peak(int32_t ab_type, int32_t pair, int32_t k_blocks, int32_t reps,
                                 double* tflops, double* ms_per_launch) {
   if (!tflops || k_blocks < 32 || k_blocks % 32 || reps < 1) return FRISK_ERR_INVALID_ARGUMENT;
-  if (!elem_size(ab_type) || ab_type == FRISK_DT_I8) return FRISK_ERR_UNSUPPORTED;   // fp32 is measured as kind::tf32
+  if (!elem_size(ab_type)) return FRISK_ERR_UNSUPPORTED;   // fp32 is measured as kind::tf32
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
@@ -1938,7 +1956,7 @@ int frisk_b200_measure_mma_peak(int32_t ab_type, int32_t pair, int32_t k_blocks,
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const uint32_t kind = is_fp8(ab_type) ? 1u : ab_type == FRISK_DT_F32 ? 2u : 0u;
+    const uint32_t kind = is_fp8(ab_type) ? 1u : ab_type == FRISK_DT_F32 ? 2u : ab_type == FRISK_DT_I8 ? 3u : 0u;
     if (pair)
       return cudaLaunchKernelEx(&cfg, frisk::mma_peak_kernel<1>, (uint32_t)k_blocks, idesc, kind, es, status);
     return cudaLaunchKernelEx(&cfg, frisk::mma_peak_kernel<0>, (uint32_t)k_blocks, idesc, kind, es, status);

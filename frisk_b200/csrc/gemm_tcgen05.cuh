@@ -24,6 +24,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ptx_sm100.cuh"
 
 namespace frisk {
@@ -294,6 +296,40 @@ __device__ __forceinline__ float cast_in<__nv_bfloat16>(__nv_bfloat16 v) {
   return __bfloat162float(v);
 }
 
+// Raw 32-bit integer sums as a "C type": the planes of an integer product split over K.
+template <>
+__device__ __forceinline__ int32_t cast_out<int32_t>(float v) { return (int32_t)v; }
+template <>
+__device__ __forceinline__ float cast_in<int32_t>(int32_t v) { return (float)v; }
+
+// Integer accumulators (kInt kernels) become fp32 bits, one rounding each, once their sum is
+// complete: partial sums travel, and are added, as integers, so a split over K changes no bit.
+template <bool kInt, int NC>
+__device__ __forceinline__ void sums_to_f32(uint32_t (&v)[NC]) {
+  if constexpr (kInt) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) v[j] = __float_as_uint(__int2float_rn((int32_t)v[j]));
+  }
+}
+template <bool kInt>
+__device__ __forceinline__ float4 sums_to_f32(float4 s) {
+  if constexpr (kInt)
+    return make_float4(__int2float_rn(__float_as_int(s.x)), __int2float_rn(__float_as_int(s.y)),
+                       __int2float_rn(__float_as_int(s.z)), __int2float_rn(__float_as_int(s.w)));
+  return s;
+}
+template <bool kInt>
+__device__ __forceinline__ float add_sums(float a, float b) {
+  if constexpr (kInt) return __int_as_float(__float_as_int(a) + __float_as_int(b));
+  return a + b;
+}
+
+// One accumulator into an element of C (an integer plane takes it as it is).
+template <typename TC>
+__device__ __forceinline__ TC scale_cast(uint32_t acc, float scale) { return cast_out<TC>(__uint_as_float(acc) * scale); }
+template <>
+__device__ __forceinline__ int32_t scale_cast<int32_t>(uint32_t acc, float) { return (int32_t)acc; }
+
 // The epilogue's view of the kernel parameters.  Every role copies what its loop needs out of the
 // __grid_constant__ parameter block into plain locals first: the block is read through its address,
 // and the inline-PTX statements clobber memory, so a field left in the block would be re-fetched
@@ -524,21 +560,21 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
     if (x.rr_kind == 1u) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const TC o = cast_out<TC>(__uint_as_float(acc[j]) * rs);
+        const TC o = scale_cast<TC>(acc[j], rs);
         out[j / kPerVec].e[j % kPerVec] = o;
         red += cast_in<TC>(o);
       }
     } else if (x.rr_kind == 3u) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const TC o = cast_out<TC>(__uint_as_float(acc[j]) * rs);
+        const TC o = scale_cast<TC>(acc[j], rs);
         out[j / kPerVec].e[j % kPerVec] = o;
         red = fminf(red, cast_in<TC>(o));
       }
     } else {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        const TC o = cast_out<TC>(__uint_as_float(acc[j]) * rs);
+        const TC o = scale_cast<TC>(acc[j], rs);
         out[j / kPerVec].e[j % kPerVec] = o;
         red = fmaxf(red, cast_in<TC>(o));
       }
@@ -547,13 +583,16 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
     if (!p.col_scale) {
 #pragma unroll
       for (int j = 0; j < NC; ++j)
-        out[j / kPerVec].e[j % kPerVec] = cast_out<TC>(__uint_as_float(acc[j]) * rs);
+        out[j / kPerVec].e[j % kPerVec] = scale_cast<TC>(acc[j], rs);
     } else {
       const float* cs = p.col_scale + col0;
 #pragma unroll
       for (int j = 0; j < NC; ++j)
         out[j / kPerVec].e[j % kPerVec] = cast_out<TC>(__uint_as_float(acc[j]) * rs * __ldg(cs + j));
     }
+  } else if constexpr (std::is_same_v<TC, int32_t>) {   // a plane: raw sums, never scaled, added to or folded
+#pragma unroll
+    for (int j = 0; j < NC; ++j) out[j / kPerVec].e[j % kPerVec] = scale_cast<TC>(acc[j], rs);
   } else {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
@@ -622,7 +661,7 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
 // The warp's 32 rows of one work item: `cols_item` columns from D column `col0`, accumulator
 // rows at tensor-memory address `t_row`.  Columns are taken 128 bytes of C at a time; the
 // tensor-memory loads of a piece are issued together and waited for once.
-template <typename TC>
+template <typename TC, bool kInt = false>
 __device__ __forceinline__ void epilogue_item(const EpiArgs& ep, EpiExt& ex, uint32_t stage,
                                               uint32_t lane, uint32_t warp_row0, uint32_t col0,
                                               uint32_t cols_item, uint32_t t_row, float& red) {
@@ -633,6 +672,7 @@ __device__ __forceinline__ void epilogue_item(const EpiArgs& ep, EpiExt& ex, uin
     for (int h = 0; h < CH / 32; ++h)
       ptx::tmem_ld_32x32b_x32(t_row + cc + 32u * h, reinterpret_cast<uint32_t(&)[32]>(v[32 * h]));
     ptx::tmem_ld_wait();
+    if constexpr (!std::is_same_v<TC, int32_t>) sums_to_f32<kInt>(v);
     epilogue_chunk<TC, CH>(ep, ex, stage, lane, warp_row0, col0 + cc, v, red);
   }
 }
@@ -685,6 +725,7 @@ __device__ __forceinline__ void slot_store(float* slot, uint32_t tile_rows, uint
 
 // Sums, in CTA order (so the result does not depend on who arrives last), every partial of
 // `tile` for 16 columns of one row.
+template <bool kInt>
 __device__ __forceinline__ void reduce_slots_x16(const float* ws, uint32_t tile, uint32_t num_kb,
                                                  uint32_t total_units, uint32_t grid,
                                                  uint32_t max_items, uint32_t tile_rows,
@@ -705,10 +746,11 @@ __device__ __forceinline__ void reduce_slots_x16(const float* ws, uint32_t tile,
     const uint32_t first_tile = b / num_kb;
     const float* slot = ws + (size_t)(c * max_items + (tile - first_tile)) * tile_elems;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum[j] += __ldcg(slot + (size_t)(c0 + j) * tile_rows + r_local);
+    for (int j = 0; j < 16; ++j) sum[j] = add_sums<kInt>(sum[j], __ldcg(slot + (size_t)(c0 + j) * tile_rows + r_local));
   }
 #pragma unroll
   for (int j = 0; j < 16; ++j) acc[j] = __float_as_uint(sum[j]);
+  sums_to_f32<kInt>(acc);
 }
 
 // Most partials of one tile the vector reduction handles; a tile with more (a grid much larger
@@ -777,7 +819,7 @@ __device__ __forceinline__ void store_rows4(const EpiArgs& p, uint32_t row, uint
 // Sums the listed slots, in list order (so the result does not depend on who arrives last), and
 // writes the tile to C.  Called by the 128 epilogue threads (tid 0 .. 127); each handles float4
 // pieces tid, tid + 128, ... of the [column][row] slot image, 4 pieces x 8 slots in flight.
-template <typename TC>
+template <typename TC, bool kInt>
 __device__ __forceinline__ void reduce_tile(const EpiArgs& p, const uint32_t* slots, uint32_t n,
                                             uint32_t tile_rows, uint32_t tile_elems,
                                             uint32_t row0, uint32_t col0, uint32_t tid) {
@@ -803,10 +845,10 @@ __device__ __forceinline__ void reduce_tile(const EpiArgs& p, const uint32_t* sl
         if (k0 + kk < n) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            sum[i].x += x[kk][i].x;
-            sum[i].y += x[kk][i].y;
-            sum[i].z += x[kk][i].z;
-            sum[i].w += x[kk][i].w;
+            sum[i].x = add_sums<kInt>(sum[i].x, x[kk][i].x);
+            sum[i].y = add_sums<kInt>(sum[i].y, x[kk][i].y);
+            sum[i].z = add_sums<kInt>(sum[i].z, x[kk][i].z);
+            sum[i].w = add_sums<kInt>(sum[i].w, x[kk][i].w);
           }
         }
       }
@@ -814,7 +856,7 @@ __device__ __forceinline__ void reduce_tile(const EpiArgs& p, const uint32_t* sl
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t e = (v0 + i * 128u) << 2;
-      store_rows4<TC>(p, row0 + (e & (tile_rows - 1u)), col0 + (e >> row_shift), sum[i]);
+      store_rows4<TC>(p, row0 + (e & (tile_rows - 1u)), col0 + (e >> row_shift), sums_to_f32<kInt>(sum[i]));
     }
   }
 }
@@ -831,7 +873,7 @@ __device__ __forceinline__ void cluster_push(uint32_t dst, uint32_t col_stride_b
   for (int j = 0; j < NC; ++j) ptx::st_shared_cluster_u32(dst + (c0 + j) * col_stride_bytes, acc[j]);
 }
 
-template <typename TC>
+template <typename TC, bool kInt>
 __device__ __forceinline__ void reduce_share(const EpiArgs& p, uint32_t buf, uint32_t cluster_k,
                                              uint32_t rank, uint32_t share, uint32_t tile_n,
                                              uint32_t row0, uint32_t col0, uint32_t tid) {
@@ -850,13 +892,13 @@ __device__ __forceinline__ void reduce_share(const EpiArgs& p, uint32_t buf, uin
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       if (k < (int)cluster_k) {
-        sum.x += x[k].x;
-        sum.y += x[k].y;
-        sum.z += x[k].z;
-        sum.w += x[k].w;
+        sum.x = add_sums<kInt>(sum.x, x[k].x);
+        sum.y = add_sums<kInt>(sum.y, x[k].y);
+        sum.z = add_sums<kInt>(sum.z, x[k].z);
+        sum.w = add_sums<kInt>(sum.w, x[k].w);
       }
     }
-    store_rows4<TC>(p, row0 + rank * share + 4u * q, col0 + col, sum);
+    store_rows4<TC>(p, row0 + rank * share + 4u * q, col0 + col, sums_to_f32<kInt>(sum));
   }
 }
 
@@ -864,7 +906,8 @@ __device__ __forceinline__ void reduce_share(const EpiArgs& p, uint32_t buf, uin
 // none of it: with the slot reduction inlined the kernel needs 200+ registers and measurably slows
 // the whole-tile main loop (8192^3 bf16: 0.98 ms against 0.83 ms), so the two are kept apart.
 // kTf32 (whole tiles, C fp32) issues kind::tf32 MMAs: the 3xTF32 plan of fp32 GEMMs.
-template <typename TC, bool kSplit, bool kTf32 = false>
+// kInt issues kind::i8 MMAs: signed 8-bit integers into 32-bit integer sums.
+template <typename TC, bool kSplit, bool kTf32 = false, bool kInt = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
                     const __grid_constant__ CUtensorMap tmap_b,
@@ -1104,6 +1147,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
                 ready = __all_sync(0xffffffffu, ptx::mbar_test_wait(full0 + 8 * next_stage, next_phase));
               if (kTf32) {
                 if (ptx::elect_one()) ptx::mma_tf32(d_base, adesc, bdesc, idesc, accumulate);
+              } else if (kInt) {
+                if (ptx::elect_one()) ptx::mma_i8(d_base, adesc, bdesc, idesc, accumulate);
+                if (mi > 1 && ptx::elect_one())
+                  ptx::mma_i8(d_base + tile_n, adesc + (a_sub_stride >> 4), bdesc, idesc, accumulate);
               } else if (kind_f8) {
                 if (ptx::elect_one()) ptx::mma_f8(d_base, adesc, bdesc, idesc, accumulate);
                 if (mi > 1 && ptx::elect_one())
@@ -1185,7 +1232,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
         ptx::tc_fence_after();
         const uint32_t t_row = tmem_base + ((quarter * 32u) << 16) + acc * tile_n;
         float red = fold_identity(rf.kind);
-        epilogue_item<TC>(ep, ex, stage_area, lane, tr * 128u + quarter * 32u, tc * tile_n, tile_n,
+        epilogue_item<TC, kInt>(ep, ex, stage_area, lane, tr * 128u + quarter * 32u, tc * tile_n, tile_n,
                           t_row, red);
         ptx::tc_fence_before();
         __syncwarp();
@@ -1279,7 +1326,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
             ptx::tmem_ld_wait();
             if (to_smem) cluster_push<32>(push_dst, share * 4u, cc, v);
             else if (to_slot) slot_store<32>(slot, tile_rows, r_local, cc, v);
-            else epilogue_store<TC, 32>(ep_item, row, tc * tile_n + cc, v);
+            else {
+              sums_to_f32<kInt>(v);
+              epilogue_store<TC, 32>(ep_item, row, tc * tile_n + cc, v);
+            }
           }
         } else {
           for (uint32_t cc = 0; cc < tile_n; cc += 16) {
@@ -1288,7 +1338,10 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
             ptx::tmem_ld_wait();
             if (to_smem) cluster_push<16>(push_dst, share * 4u, cc, v);
             else if (to_slot) slot_store<16>(slot, tile_rows, r_local, cc, v);
-            else epilogue_store<TC, 16>(ep_item, row, tc * tile_n + cc, v);
+            else {
+              sums_to_f32<kInt>(v);
+              epilogue_store<TC, 16>(ep_item, row, tc * tile_n + cc, v);
+            }
           }
         }
       }
@@ -1312,7 +1365,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
         if (last_flag) {
           __threadfence();
           if (contrib_n <= kMaxContrib) {
-            reduce_tile<TC>(ep_item, contrib_slots, contrib_n, tile_rows, tile_elems,
+            reduce_tile<TC, kInt>(ep_item, contrib_slots, contrib_n, tile_rows, tile_elems,
                             tr * tile_rows, tc * tile_n, threadIdx.x - 64u);
           } else {
             for (uint32_t sub = 0; sub < mi; ++sub) {
@@ -1320,7 +1373,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
               const uint32_t row = tr * tile_rows + r_local;
               for (uint32_t cc = 0; cc < tile_n; cc += 16) {
                 uint32_t v[16];
-                reduce_slots_x16(ep.ws, work.tile, num_kb_all, total_units, gridDim.x, max_items,
+                reduce_slots_x16<kInt>(ep.ws, work.tile, num_kb_all, total_units, gridDim.x, max_items,
                                  tile_rows, tile_elems, r_local, cc, v);
                 epilogue_store<TC, 16>(ep_item, row, tc * tile_n + cc, v);
               }
@@ -1355,7 +1408,7 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
         tile_coords(group_r, tiles_r, tiles_c, blockIdx.x >> cluster_sh, tr, tc);
         EpiArgs ep_out = ep;
         ep_out.split_mode = 0;
-        reduce_share<TC>(ep_out, red_base, cluster_k, my_rank, share, tile_n, tr * tile_rows,
+        reduce_share<TC, kInt>(ep_out, red_base, cluster_k, my_rank, share, tile_n, tr * tile_rows,
                          tc * tile_n, threadIdx.x - 64u);
       }
       FRISK_STAMP(threadIdx.x == 64, 327);
@@ -1440,7 +1493,8 @@ __global__ void splitk_finalize_kernel(float* __restrict__ ws, int64_t ws_ld, TC
 // (+ C)), the planes summed in their order, four columns per thread.  `ldp` (the planes' pitch) is
 // a multiple of 4; `vec_ok`: four elements of C at a column that is a multiple of 4 may leave as
 // one store.  Launched as a programmatic dependent of the GEMM, like row_fold_finalize_kernel.
-template <typename TC>
+// kInt: the planes hold 32-bit integers, added as such and converted once.
+template <typename TC, bool kInt>
 __global__ void __launch_bounds__(256) kplanes_sum_kernel(const float* __restrict__ planes,
                                                           uint64_t plane_elems, uint32_t parts,
                                                           int64_t ldp, TC* __restrict__ C, int64_t ldc,
@@ -1462,8 +1516,12 @@ __global__ void __launch_bounds__(256) kplanes_sum_kernel(const float* __restric
 #pragma unroll 8
     for (uint32_t z = 1; z < parts; ++z) {
       const float4 t = __ldcg(reinterpret_cast<const float4*>(src + (size_t)z * plane_elems));
-      s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+      s.x = add_sums<kInt>(s.x, t.x);
+      s.y = add_sums<kInt>(s.y, t.y);
+      s.z = add_sums<kInt>(s.z, t.z);
+      s.w = add_sums<kInt>(s.w, t.w);
     }
+    s = sums_to_f32<kInt>(s);
     float v[4] = {s.x, s.y, s.z, s.w};
     const float sm = scale_m ? __ldg(scale_m + m) : 1.0f;
     TC* dst = C + m * ldc + n0;

@@ -49,7 +49,8 @@ __device__ __forceinline__ PairItem pair_item(uint32_t i, uint32_t narrow_from, 
 }
 
 // kTf32 (C fp32 only) issues kind::tf32 MMAs on fp32 operand tiles: the 3xTF32 plan of fp32 GEMMs.
-template <typename TC, bool kTf32 = false>
+// kInt issues kind::i8 MMAs (TC = int32_t: the planes of an integer product split over K).
+template <typename TC, bool kTf32 = false, bool kInt = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                          const __grid_constant__ CUtensorMap tmap_b,
@@ -271,6 +272,8 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
               ready = __all_sync(0xffffffffu, ptx::mbar_test_wait(full0 + 8 * next_stage, next_phase));
             if (kTf32) {
               if (ptx::elect_one()) ptx::mma_tf32_pair(d_base, adesc, bdesc, idesc, accumulate);
+            } else if (kInt) {
+              if (ptx::elect_one()) ptx::mma_i8_pair(d_base, adesc, bdesc, idesc, accumulate);
             } else if (kind_f8) {
               if (ptx::elect_one()) ptx::mma_f8_pair(d_base, adesc, bdesc, idesc, accumulate);
             } else {
@@ -346,7 +349,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
       const uint32_t warp_row0 = tr * 256u + rank * 128u + quarter * 32u;
       const uint32_t t_row = tmem_base + ((quarter * 32u) << 16) + acc * tile_n;
       float red = fold_identity(rf.kind);
-      epilogue_item<TC>(ep, ex, stage_area, lane, warp_row0, col0, cols_item, t_row, red);
+      epilogue_item<TC, kInt>(ep, ex, stage_area, lane, warp_row0, col0, cols_item, t_row, red);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(leader_acc_empty0 + 8 * acc);

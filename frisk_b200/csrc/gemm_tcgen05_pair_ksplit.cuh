@@ -18,7 +18,7 @@
 
 namespace frisk {
 
-template <typename TC>
+template <typename TC, bool kInt = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tcgen05_pair_ksplit_kernel(const __grid_constant__ CUtensorMap tmap_a,
                                 const __grid_constant__ CUtensorMap tmap_b,
@@ -160,7 +160,9 @@ gemm_tcgen05_pair_ksplit_kernel(const __grid_constant__ CUtensorMap tmap_a,
           const uint64_t bdesc = bdesc0 + (uint64_t)((ks * b_k_step) >> 4);
           const uint64_t adesc = adesc0 + (uint64_t)((ks * a_k_step) >> 4);
           const uint32_t accumulate = first | (ks > 0 ? 1u : 0u);
-          if (kind_f8) {
+          if (kInt) {
+            if (ptx::elect_one()) ptx::mma_i8_pair(tmem_base, adesc, bdesc, idesc, accumulate);
+          } else if (kind_f8) {
             if (ptx::elect_one()) ptx::mma_f8_pair(tmem_base, adesc, bdesc, idesc, accumulate);
           } else {
             if (ptx::elect_one()) ptx::mma_f16_pair(tmem_base, adesc, bdesc, idesc, accumulate);
@@ -255,12 +257,13 @@ gemm_tcgen05_pair_ksplit_kernel(const __grid_constant__ CUtensorMap tmap_a,
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 x = ptx::ld_shared_f32x4(mine + slot * img_bytes + (cc + 4u * i) * 4u);
-            v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + x.x);
-            v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + x.y);
-            v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + x.z);
-            v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + x.w);
+            v[4 * i] = __float_as_uint(add_sums<kInt>(__uint_as_float(v[4 * i]), x.x));
+            v[4 * i + 1] = __float_as_uint(add_sums<kInt>(__uint_as_float(v[4 * i + 1]), x.y));
+            v[4 * i + 2] = __float_as_uint(add_sums<kInt>(__uint_as_float(v[4 * i + 2]), x.z));
+            v[4 * i + 3] = __float_as_uint(add_sums<kInt>(__uint_as_float(v[4 * i + 3]), x.w));
           }
         }
+        sums_to_f32<kInt>(v);
         epilogue_store<TC, 32>(ep, row, tc * tile_n + cc, v);
       }
       ptx::tc_fence_before();

@@ -130,3 +130,127 @@ def test_oracle_agrees_with_the_exact_product():
     prod, want = expect(a, b, sa, sb)
     check(ref.ref_gemm(w, acc64=True), prod, want, W.F32)
     check(R.gemm_host(w), prod, want, W.F32)
+
+
+# ----------------------------------------------------------------------------- tensor-core plans
+# Every plan family, over the whole range of the type: without scales an fp32 C is the exact sum
+# rounded once, whatever the tiles and the split of K.
+PLANS = [
+    # (M, N, K, kernel, plan options)
+    (256, 512, 256, "tcgen05_pair", {}),
+    (300, 520, 272, "tcgen05_pair", {}),                                 # ragged rows, columns and K
+    (700, 1000, 4112, "tcgen05_pair", {"k_split": -1}),                  # many k-blocks, narrow last wave
+    (512, 768, 640, "tcgen05_pair", {"epilogue": 1}),
+    (512, 768, 640, "tcgen05_pair", {"epilogue": 2}),
+    (512, 768, 640, "tcgen05_pair", {"epilogue": 3}),
+    (512, 768, 640, "tcgen05_pair", {"epilogue": 4}),
+    (128, 256, 256, "tcgen05", {"force_kernel": "tcgen05"}),
+    (333, 200, 400, "tcgen05", {"force_kernel": "tcgen05", "tile_n": 64}),
+    (1, 4096, 4096, "skinny", {}),                                       # one token
+    (1, 256, 16, "skinny", {}),
+    (16, 8192, 1024, "skinny", {}),
+    (33, 4100, 528, "skinny", {}),
+    (64, 2048, 2048, "skinny", {}),
+    (100, 8192, 512, "skinny", {}),
+    (128, 8192, 1040, "skinny", {}),
+    (16, 512, 4096, "skinny", {}),
+    (16, 8192, 1024, "skinny", {"num_ctas": 97}),                        # stream-K: partials in slots
+    (24, 512, 8192, "skinny", {"num_ctas": 148}),                        # more partials of a tile than its list holds
+    (512, 512, 4096, "tcgen05_pair", {"k_split": 3}),                    # K over the pairs of a cluster
+    (260, 128, 8192, "tcgen05_pair", {"k_split": 3}),
+    (512, 500, 4096, "tcgen05_pair", {"k_split": 2}),                    # K planes
+    (520, 264, 2320, "tcgen05_pair", {"k_split": 2}),
+    (129, 1000, 8192, "tcgen05", {"k_split": 1}),                        # K over a cluster, not swapped
+    (512, 512, 65536, "tcgen05_pair", {}),
+]
+
+
+@pytest.mark.parametrize("M,N,K,kernel,kw", PLANS, ids=["-".join(map(str, [*p[:3], *p[4].values()])) for p in PLANS])
+def test_sums_are_exact_on_every_plan(M, N, K, kernel, kw):
+    a, b, _, _ = make(M, N, K, 7, full=True)
+    c = np.zeros((M, N), np.float32)
+    plan = R.GemmPlan(M, N, K, W.I8, W.F32, transB=True, **kw)
+    assert plan.info["kernel_name"] == kernel, plan.info
+    plan.run_host(a, np.ascontiguousarray(b.T), c)
+    plan.close()
+    want = np.rint(a.astype(np.float64) @ b.astype(np.float64))
+    assert np.array_equal(c, want.astype(np.float32))
+
+
+@pytest.mark.parametrize("clear", [True, False], ids=["set", "add"])
+@pytest.mark.parametrize("ct", [W.F32, W.F16, W.BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,kernel,kw", PLANS, ids=["-".join(map(str, [*p[:3], *p[4].values()])) for p in PLANS])
+def test_scales_and_result_types_on_every_plan(M, N, K, kernel, kw, ct, clear):
+    run(M, N, K, ct, clear=clear, seed=8, kernel=kernel, **kw)
+
+
+@pytest.mark.parametrize("kind", ["max", "add", "min"])
+@pytest.mark.parametrize("M,N,K", [(300, 520, 272), (512, 768, 640)])
+def test_row_reduce_folded_into_the_epilogue(M, N, K, kind):
+    a, b, sa, sb = make(M, N, K, 9)
+    c, dst = np.zeros((M, N), np.uint16), np.zeros(M, np.uint16)
+    plan = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True, row_reduce=kind)
+    plan.run_host(a, np.ascontiguousarray(b.T), c, sa, sb, dst)
+    plan.close()
+    check(c, *expect(a, b, sa, sb), W.BF16)
+    want, mag = ref.ref_reduce(c, 1, W.BF16, kind)
+    err = np.abs(W.decode(dst, W.BF16).astype(np.float64) - want)
+    assert (err <= (0 if kind != "add" else N * U * mag + 2.0 ** -8 * np.abs(want))).all()
+
+
+def test_stays_inside_c_and_the_workspace():
+    """Device buffers with guards around C, the rows' padding and the workspace."""
+    import torch
+    dev = torch.device("cuda:0")
+    for M, N, K, kw in ((1, 300, 144, {}), (16, 8192, 1024, {"num_ctas": 97}), (130, 257, 272, {}), (512, 500, 4096, {"k_split": 2}),
+                        (300, 520, 4099, {})):
+        a, b, sa, sb = make(M, N, K, 10)
+        for ct, ldc in ((W.BF16, N + 3), (W.F32, N + 4)):
+            es = W.ELEM_SIZE[ct]
+            plan = R.GemmPlan(M, N, K, W.I8, ct, transB=True, scales=True, ldc=ldc, **kw)
+            guard = 256
+            cbuf = torch.full((M * ldc * es + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
+            wbuf = torch.full((plan.workspace_bytes + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
+            A, B = torch.from_numpy(a).to(dev), torch.from_numpy(np.ascontiguousarray(b.T)).to(dev)
+            dsa, dsb = torch.from_numpy(sa).to(dev), torch.from_numpy(sb).to(dev)
+            plan.run(A, B, cbuf.data_ptr() + guard, dsa, dsb, wbuf[guard:guard + plan.workspace_bytes] if plan.workspace_bytes else None,
+                     stream=torch.cuda.current_stream().cuda_stream)
+            torch.cuda.synchronize()
+            host, ws = cbuf.cpu().numpy(), wbuf.cpu().numpy()
+            assert (host[:guard] == 0x5A).all() and (host[guard + M * ldc * es:] == 0x5A).all()
+            assert (ws[:guard] == 0x5A).all() and (ws[guard + plan.workspace_bytes:] == 0x5A).all()
+            rows = host[guard:guard + M * ldc * es].reshape(M, ldc * es)
+            assert (rows[:, N * es:] == 0x5A).all()
+            check(np.ascontiguousarray(rows[:, :N * es]).view(W.storage_numpy_dtype(ct)), *expect(a, b, sa, sb), ct)
+            plan.close()
+
+
+def test_captured_into_a_graph():
+    import torch
+    dev = torch.device("cuda:0")
+    M, N, K = 16, 1024, 2048
+    plan = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True)
+    A, B = torch.zeros((M, K), dtype=torch.int8, device=dev), torch.zeros((N, K), dtype=torch.int8, device=dev)
+    sa, sb = torch.zeros(M, device=dev), torch.zeros(N, device=dev)
+    c = torch.zeros((M, N), dtype=torch.bfloat16, device=dev)
+    ws = torch.zeros(max(plan.workspace_bytes, 16), dtype=torch.uint8, device=dev)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        plan.run(A, B, c, sa, sb, ws, stream=side.cuda_stream)
+    for seed in (11, 12):
+        a, b, ha, hb = make(M, N, K, seed)
+        A.copy_(torch.from_numpy(a))
+        B.copy_(torch.from_numpy(np.ascontiguousarray(b.T)))
+        sa.copy_(torch.from_numpy(ha))
+        sb.copy_(torch.from_numpy(hb))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(c.view(torch.int16).cpu().numpy().view(np.uint16), *expect(a, b, ha, hb), W.BF16)
+    plan.close()
+
+
+def test_the_tensor_pipes_rate_can_be_measured():
+    got = R.measure_mma_peak(W.I8, pair=True, k_blocks=1024, reps=5)
+    assert got["tflops"] > 1000.0, got
+    print(got)

@@ -57,3 +57,14 @@ def test_builder_and_parser_take_8_bit_integers():
         tys = [h64.memref_type((8, 4), "int64"), h64.memref_type((4, 16), "int64"), h64.memref_type((8, 16), "bf16")]
         _, e = h64.new_kernel("k", tys)
         h64.builder.create_gemm_op(*[e.get_argument(i) for i in range(3)])
+
+
+def test_kernel_families_and_the_fixed_scratch_entry_point():
+    for (M, N, K), kernel in (((8192, 8192, 8192), "tcgen05_pair"), ((16, 8192, 8192), "skinny"), ((1, 4096, 4096), "skinny"),
+                              ((128, 192, 256), "tcgen05")):
+        p = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True)
+        assert p.info["kernel_name"] == kernel and p.info["tile_k"] == 128, p.info
+        p.close()
+    d = R.GemmDesc()     # its scratch adds fp32 partial sums: not for an exact product
+    d.M, d.N, d.K, d.a_type, d.b_type, d.c_type, d.transB, d.clear_accum = 16, 512, 512, W.I8, W.I8, W.BF16, 1, 1
+    assert R.lib().frisk_b200_gemm_skinny_static(d, 0x10000, 0x20000, 0x30000, None, None, None, None) == -2
