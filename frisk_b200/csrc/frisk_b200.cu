@@ -1082,11 +1082,15 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
   memset(&pl->info, 0, sizeof pl->info);
   int dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess) {
-    cudaDeviceProp prop;
-    if (cudaGetDeviceProperties(&prop, dev) == cudaSuccess) {
+    // (two attributes: the whole property structure takes milliseconds to fill)
+    int major = 0, sms = 0;
+    if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) == cudaSuccess &&
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) {
       pl->device = dev;
-      pl->sm_count = prop.multiProcessorCount;
-      pl->have_device = prop.major == 10;
+      pl->sm_count = sms;
+      pl->have_device = major == 10;
+    } else {
+      cudaGetLastError();
     }
   } else {
     cudaGetLastError();  // plans can be made (and inspected) on a machine without a GPU

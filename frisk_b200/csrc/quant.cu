@@ -46,30 +46,54 @@ int check_desc(const frisk_quant_desc& d) {
   return FRISK_OK;
 }
 
-template <typename TIn, typename TW, int QT, int KIND>
-cudaError_t launch(const Params& p, int64_t ctas, cudaStream_t st) {
-  frisk_quant::quant_rows_generic_kernel<TIn, TW, QT, KIND><<<(unsigned)ctas, 256, 0, st>>>(p);
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether every row of a buffer at `ptr` with row pitch `ld` (elements of `es` bytes) starts on a
+// multiple of `to` bytes.  A buffer that is not there does.
+bool rows_on(const void* ptr, int64_t ld, int es, int to) {
+  return !ptr || (reinterpret_cast<uintptr_t>(ptr) % to == 0 && (ld * es) % to == 0);
+}
+
+constexpr int kMaxGroups = 4;   // groups of eight elements a thread holds at most
+
+template <typename TIn, typename TW, int KIND>
+cudaError_t launch(Params p, int sms, cudaStream_t st) {
+  const int es = sizeof(TIn);
+  const bool aligned = p.cols % 8 == 0 && rows_on(p.x, p.ldx, es, 16) && rows_on(p.other, p.ldo, es, 16) &&
+                       rows_on(p.sum_out, p.lds, es, 16) && rows_on(p.q, p.ldq, 1, 8) && rows_on(p.weight, 0, 1, 16);
+  const int64_t groups = p.cols / 8;
+  if (!aligned || groups > 1024 * kMaxGroups) {
+    frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND>
+        <<<(unsigned)std::min<int64_t>(p.rows, 0x7fffffff), 256, 0, st>>>(p);
+    return cudaGetLastError();
+  }
+  // Many rows: four groups a thread, the most loads in flight per warp that registers allow; few rows:
+  // one, so that a row is spread over as many threads as there are.
+  const bool few = p.rows < 2 * (int64_t)sms;
+  int nv = few ? 1 : kMaxGroups;
+  while (ceil_div(groups, 32 * nv) > 32) nv *= 2;
+  while (nv > 1 && 32 * (nv / 2) >= groups) nv /= 2;   // short rows: no more than a warp can use
+  p.warps_per_row = (int)ceil_div(groups, 32 * nv);
+  p.rows_per_cta = std::max(1, 8 / p.warps_per_row);
+  const int64_t ctas = ceil_div(p.rows, p.rows_per_cta);
+  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+  const unsigned threads = 32u * p.warps_per_row * p.rows_per_cta;
+  switch (nv) {
+    case 1: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 1><<<(unsigned)ctas, threads, 0, st>>>(p); break;
+    case 2: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 2><<<(unsigned)ctas, threads, 0, st>>>(p); break;
+    default: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 4><<<(unsigned)ctas, threads, 0, st>>>(p); break;
+  }
   return cudaGetLastError();
 }
 
-template <typename TIn, int QT>
-cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, cudaStream_t st) {
-  const int64_t ctas = std::min<int64_t>(d.rows, 0x7fffffff);
-  switch (d.kind) {
-    case FRISK_QUANT_PLAIN: return launch<TIn, TIn, QT, FRISK_QUANT_PLAIN>(p, ctas, st);
-    case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, QT, FRISK_QUANT_SILU_MUL>(p, ctas, st);
-    default:
-      return d.weight_type == d.in_type ? launch<TIn, TIn, QT, FRISK_QUANT_RMSNORM>(p, ctas, st)
-                                        : launch<TIn, float, QT, FRISK_QUANT_RMSNORM>(p, ctas, st);
-  }
-}
-
 template <typename TIn>
-cudaError_t launch_q(const frisk_quant_desc& d, const Params& p, cudaStream_t st) {
-  switch (d.q_type) {
-    case FRISK_DT_I8: return launch_kind<TIn, FRISK_DT_I8>(d, p, st);
-    case FRISK_DT_E4M3: return launch_kind<TIn, FRISK_DT_E4M3>(d, p, st);
-    default: return launch_kind<TIn, FRISK_DT_E5M2>(d, p, st);
+cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, int sms, cudaStream_t st) {
+  switch (d.kind) {
+    case FRISK_QUANT_PLAIN: return launch<TIn, TIn, FRISK_QUANT_PLAIN>(p, sms, st);
+    case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, FRISK_QUANT_SILU_MUL>(p, sms, st);
+    default:
+      return d.weight_type == d.in_type ? launch<TIn, TIn, FRISK_QUANT_RMSNORM>(p, sms, st)
+                                        : launch<TIn, float, FRISK_QUANT_RMSNORM>(p, sms, st);
   }
 }
 
@@ -95,6 +119,7 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
   p.lds = d.lds ? d.lds : d.cols;
   p.ldq = d.ldq ? d.ldq : d.cols;
   p.eps = d.eps;
+  p.q_type = d.q_type;
   if (d.rows == 0) return FRISK_OK;
   if (!args->x || !args->q || !args->scale) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: null x, q or scale");
   const int es = in_bytes(d.in_type), ws = in_bytes(norm ? d.weight_type : d.in_type);
@@ -117,10 +142,15 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
     if (prev != d.device && (e = cudaSetDevice(d.device)) != cudaSuccess) return fail_cuda(e, "cudaSetDevice");
   }
   cudaStream_t st = static_cast<cudaStream_t>(args->stream);
-  switch (d.in_type) {
-    case FRISK_DT_F32: e = launch_q<float>(d, p, st); break;
-    case FRISK_DT_F16: e = launch_q<__half>(d, p, st); break;
-    default: e = launch_q<__nv_bfloat16>(d, p, st); break;
+  int dev = d.device, sms = 0;
+  e = dev >= 0 ? cudaSuccess : cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) {
+    switch (d.in_type) {
+      case FRISK_DT_F32: e = launch_kind<float>(d, p, sms, st); break;
+      case FRISK_DT_F16: e = launch_kind<__half>(d, p, sms, st); break;
+      default: e = launch_kind<__nv_bfloat16>(d, p, sms, st); break;
+    }
   }
   if (prev >= 0 && prev != d.device) cudaSetDevice(prev);
   if (e != cudaSuccess) return fail_cuda(e, "quant kernel launch");

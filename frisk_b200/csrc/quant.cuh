@@ -36,6 +36,8 @@ struct Params {
   int64_t rows, cols;
   int64_t ldx, ldo, lds, ldq;
   float eps;
+  int32_t q_type;
+  int32_t warps_per_row, rows_per_cta;   // quant_rows_kernel
 };
 
 template <typename T>
@@ -55,45 +57,60 @@ __device__ __forceinline__ __half from_float<__half>(float v) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-template <int QT>
-__device__ __forceinline__ constexpr float q_max() {
-  return QT == FRISK_DT_I8 ? 127.f : QT == FRISK_DT_E4M3 ? 448.f : 57344.f;
+// The 8-bit type is a run-time value, the same for the whole grid: it decides a few instructions per
+// group of elements, not worth three times the kernels.
+__device__ __forceinline__ float q_max(int qt) {
+  return qt == FRISK_DT_I8 ? 127.f : qt == FRISK_DT_E4M3 ? 448.f : 57344.f;
 }
-// One value of at most Q in magnitude (a little above it by rounding) into its 8 bits; NaN becomes 0
+// Values of at most Q in magnitude (a little above it by rounding) into their 8 bits; NaN becomes 0
 // in int8, which has none.
-template <int QT>
-__device__ __forceinline__ uint8_t encode8(float v) {
-  if (QT == FRISK_DT_I8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(v)));
-  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, QT == FRISK_DT_E4M3 ? __NV_E4M3 : __NV_E5M2);
+__device__ __forceinline__ uint8_t encode8(float v, int qt) {
+  if (qt == FRISK_DT_I8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(v)));
+  return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, qt == FRISK_DT_E4M3 ? __NV_E4M3 : __NV_E5M2);
 }
 
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// Sum and maximum over a warp, in every lane.
+template <int KIND>
+__device__ __forceinline__ void warp_fold(float& sum, uint32_t& mx) {
+  if (KIND == FRISK_QUANT_RMSNORM) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  }
+  mx = __reduce_max_sync(0xffffffffu, mx);
+}
+
 __device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 
-// scale and the divisor of g from the row's sum of h^2 and maximum of |g| (as bits)
-template <int KIND, int QT>
-__device__ __forceinline__ void row_scale(float sum_sq, uint32_t max_bits, int64_t cols, float eps, float* scale,
-                                          float* divisor) {
-  const float d = __fdiv_rn(__uint_as_float(max_bits), q_max<QT>());
+// scale[r] and the divisor of g from the row's sum of h^2 and maximum of |g| (as bits).  Every thread
+// of the row needs the divisor; the scale, with its root, only the one that stores it (`writer`).
+template <int KIND>
+__device__ __forceinline__ float row_divisor(float sum_sq, uint32_t max_bits, int64_t cols, float eps, int qt,
+                                             bool writer, float* scale) {
+  const float d = __fdiv_rn(__uint_as_float(max_bits), q_max(qt));
   if (KIND != FRISK_QUANT_RMSNORM) {
-    *scale = *divisor = max_bits > 0x7f800000u ? d : fmaxf(d, kTinyScale);
-    return;
+    const float s = max_bits > 0x7f800000u ? d : fmaxf(d, kTinyScale);
+    if (writer) *scale = s;
+    return s;
   }
+  // (rsqrt(..) of a finite sum is above 1e-20: a divisor of 1e-18 needs no look at the scale)
+  if (!writer && d >= 1e-18f) return d;
   // a sum of squares past the range of fp32 has no norm: NaN, not a scale of zero
   const float rstd = sum_sq < __uint_as_float(0x7f800000u)
                          ? __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps))
                          : __uint_as_float(0x7fc00000u);
   const float s = rstd * d;
-  // (a scale below 2^-126 is raised to it, and g's divisor with it; NaN fails the test and stays)
-  *scale = s < kTinyScale ? kTinyScale : s;
-  // (not to zero: g is zero or a few of fp32's smallest steps there)
-  *divisor = s < kTinyScale ? fmaxf(__fdiv_rn(kTinyScale, rstd), __uint_as_float(1u)) : d;
+  // a scale below 2^-126 is raised to it, and g's divisor with it (not to zero: g is zero or a few
+  // of fp32's smallest steps there); NaN fails the test and stays
+  const bool tiny = s < kTinyScale;
+  if (writer) *scale = tiny ? kTinyScale : s;
+  return tiny ? fmaxf(__fdiv_rn(kTinyScale, rstd), __uint_as_float(1u)) : d;
 }
 
 // The plain form of the three kinds: a CTA per row, two passes over it, element by element.  Serves
 // any type, pitch, alignment and width.
-template <typename TIn, typename TW, int QT, int KIND>
+template <typename TIn, typename TW, int KIND>
 __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p) {
   __shared__ float s_sum[8];
   __shared__ uint32_t s_max[8];
@@ -118,8 +135,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       mx = max(mx, abs_bits(value(c, &h)));
       if (KIND == FRISK_QUANT_RMSNORM) sum = fmaf(h, h, sum);
     }
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    mx = __reduce_max_sync(0xffffffffu, mx);
+    warp_fold<KIND>(sum, mx);
     if ((threadIdx.x & 31) == 0) {
       s_sum[threadIdx.x >> 5] = sum;
       s_max[threadIdx.x >> 5] = mx;
@@ -131,17 +147,180 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       sum += s_sum[i];
       mx = max(mx, s_max[i]);
     }
-    float scale, divisor;
-    row_scale<KIND, QT>(sum, mx, p.cols, p.eps, &scale, &divisor);
-    if (threadIdx.x == 0) p.scale[r] = scale;
+    const float divisor = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
     // sum_out may be x or the residual: an element is written by the thread that has just read it
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
-      q[c] = encode8<QT>(__fdiv_rn(value(c, &h), divisor));
+      q[c] = encode8(__fdiv_rn(value(c, &h), divisor), p.q_type);
       if (KIND == FRISK_QUANT_RMSNORM && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
+  }
+}
+
+// ---- rows in registers -------------------------------------------------------------------------
+// Eight neighbouring elements as they are stored: one or two 16-byte words.
+template <typename T>
+struct Eight {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* p) {   // read once: past L1
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w)
+                 : "l"(reinterpret_cast<const uint4*>(p) + i)
+                 : "memory");
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> load8_shared_by_rows(const T* p) {
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Eight<T>& r, float (&f)[8]) {
+  const T* e = reinterpret_cast<const T*>(r.w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = to_float<T>(e[j]);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  Eight<T> r;
+  T* e = reinterpret_cast<T*>(r.w);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) e[j] = from_float<T>(f[j]);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+}
+// Eight values into eight bytes.
+__device__ __forceinline__ uint2 encode8x8(const float (&v)[8], int qt) {
+  union {
+    uint2 u;
+    uint16_t h[4];
+    uint8_t b[8];
+  } r;
+  if (qt == FRISK_DT_I8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.b[j] = encode8(v[j], FRISK_DT_I8);
+  } else if (qt == FRISK_DT_E4M3) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j], v[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j], v[2 * j + 1]), __NV_SATFINITE, __NV_E5M2);
+  }
+  return r.u;
+}
+
+// v / d to nearest for many v and one d: with y the reciprocal of d to nearest and q = v y, the
+// remainder v - q d is exact in one fused multiply-add, and q plus the remainder times y is the
+// correctly rounded quotient (P. Markstein, IBM Journal of Research and Development 34(1), 1990) where
+// nothing leaves the range of normal numbers: d is at least 1e-30 here and v at most Q d.  A divisor
+// of infinity or NaN makes the values NaN, as the row's scale says.
+__device__ __forceinline__ float div_by(float v, float d, float y) {
+  const float q = v * y;
+  return fmaf(fmaf(-q, d, v), y, q);
+}
+
+// Whole rows in registers: `warps_per_row` warps share a row, every thread NV groups of eight elements
+// of it, so the row is read once and the only pause is the fold of (sum, maximum) over the warps.
+// For rows whose starts, in every buffer, allow 16-byte accesses (8 for q) and whose width is a
+// multiple of eight.  CTAs of more than one row fold them side by side.
+template <typename TIn, typename TW, int KIND, int NV>
+__global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
+  __shared__ float s_sum[32];
+  __shared__ uint32_t s_max[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wpr = p.warps_per_row;
+  const int slot = warp / wpr, warp_in_row = warp - slot * wpr;
+  const int64_t r = (int64_t)blockIdx.x * p.rows_per_cta + slot;
+  const bool live = r < p.rows;
+  const int t = warp_in_row * 32 + lane, step = wpr * 32, groups = (int)(p.cols >> 3);
+  const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
+  const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
+  const TW* w = static_cast<const TW*>(p.weight);
+  TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
+
+  Eight<TIn> rx[NV], ro[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int gidx = t + i * step;
+    if (live && gidx < groups) {
+      rx[i] = load8(x + 8 * (int64_t)gidx);
+      if (KIND != FRISK_QUANT_PLAIN && o) ro[i] = load8(o + 8 * (int64_t)gidx);
+    }
+  }
+  float g[NV][8];
+  float sum = 0.f;
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int gidx = t + i * step;
+    if (live && gidx < groups) {
+      unpack8(rx[i], g[i]);
+      if (KIND == FRISK_QUANT_SILU_MUL) {
+        float u[8];
+        unpack8(ro[i], u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[i][j] = silu_mul(g[i][j], u[j]);
+      }
+      if (KIND == FRISK_QUANT_RMSNORM) {
+        if (o) {
+          float u[8];
+          unpack8(ro[i], u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[i][j] += u[j];
+          if (so) store8(so + 8 * (int64_t)gidx, g[i]);   // read above by this thread, if it is x or the residual
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(g[i][j], g[i][j], sum);
+        if (w) {
+          float u[8];
+          unpack8(load8_shared_by_rows(w + 8 * (int64_t)gidx), u);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) g[i][j] *= u[j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mx = max(mx, abs_bits(g[i][j]));
+    }
+  }
+  warp_fold<KIND>(sum, mx);
+  if (wpr > 1) {
+    if (lane == 0) {
+      s_sum[warp] = sum;
+      s_max[warp] = mx;
+    }
+    __syncthreads();
+    sum = lane < wpr ? s_sum[slot * wpr + lane] : 0.f;
+    mx = lane < wpr ? s_max[slot * wpr + lane] : 0u;
+    warp_fold<KIND>(sum, mx);
+  }
+  if (!live) return;
+  float d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
+  if (d < 1e-30f) {   // both up by the same power of two (exact), so that div_by stays in range
+    d *= 0x1p96f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[i][j] *= 0x1p96f;
+  }
+  const float y = __frcp_rn(d);
+  uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int gidx = t + i * step;
+    if (gidx < groups) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[i][j] = div_by(g[i][j], d, y);
+      *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = encode8x8(g[i], p.q_type);
+    }
   }
 }
 
