@@ -183,39 +183,112 @@ __device__ __forceinline__ Eight<T> load8_shared_by_rows(const T* p) {
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   return r;
 }
+// Two fp32 numbers in a register pair: the packed instructions do both for one issue slot, and it is
+// issue slots that the gated kind would otherwise be bound by.
+using f2 = uint64_t;
+__device__ __forceinline__ f2 pack2(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ f2 pack2(float v) { return pack2(v, v); }
+__device__ __forceinline__ float lo2(f2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float hi2(f2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// max(|a|, |b|, m), NaN if one of them is
+__device__ __forceinline__ float abs_max(f2 v, float m) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(lo2(v)), "f"(hi2(v)), "f"(m));
+  return r;
+}
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 template <typename T>
-__device__ __forceinline__ void unpack8(const Eight<T>& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const Eight<T>& r, f2 (&f)[4]) {
   const T* e = reinterpret_cast<const T*>(r.w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = to_float<T>(e[j]);
+  for (int j = 0; j < 4; ++j) f[j] = pack2(to_float<T>(e[2 * j]), to_float<T>(e[2 * j + 1]));
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(T* p, const f2 (&f)[4]) {
   Eight<T> r;
   T* e = reinterpret_cast<T*>(r.w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) e[j] = from_float<T>(f[j]);
+  for (int j = 0; j < 4; ++j) {
+    e[2 * j] = from_float<T>(lo2(f[j]));
+    e[2 * j + 1] = from_float<T>(hi2(f[j]));
+  }
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
 // Eight values into eight bytes.
-__device__ __forceinline__ uint2 encode8x8(const float (&v)[8], int qt) {
+__device__ __forceinline__ uint2 encode8x8(const f2 (&v)[4], int qt) {
   union {
-    uint2 u;
+    uint32_t u[2];
     uint16_t h[4];
-    uint8_t b[8];
   } r;
   if (qt == FRISK_DT_I8) {
+    // (|v| rounds to 127 at most; NaN becomes 0)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r.b[j] = encode8(v[j], FRISK_DT_I8);
+    for (int j = 0; j < 2; ++j) {
+      uint32_t upper;
+      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(upper) : "r"(__float2int_rn(hi2(v[2 * j + 1]))), "r"(__float2int_rn(lo2(v[2 * j + 1]))), "r"(0));
+      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(r.u[j]) : "r"(__float2int_rn(hi2(v[2 * j]))), "r"(__float2int_rn(lo2(v[2 * j]))), "r"(upper));
+    }
   } else if (qt == FRISK_DT_E4M3) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j], v[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
+    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[j]), hi2(v[j])), __NV_SATFINITE, __NV_E4M3);
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * j], v[2 * j + 1]), __NV_SATFINITE, __NV_E5M2);
+    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[j]), hi2(v[j])), __NV_SATFINITE, __NV_E5M2);
   }
-  return r.u;
+  return make_uint2(r.u[0], r.u[1]);
+}
+
+// gate / (1 + exp(-gate)) * up for two elements.  With e = exp(-|gate|), which cannot overflow:
+//   silu = gate * (gate < 0 ? e : 1) / (1 + e).
+// e = 2^-(a log2(e)), a = |gate| (at most 200: e is 0 long before): the product is split into its
+// rounded value t, for the hardware's 2^x, and the exact rest, which with log2(e)'s own rest enters
+// to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's, corrected by its remainder
+// as in div_by.  Exponentials below 2^-126 (gates below -87) are zero.
+__device__ __forceinline__ f2 silu_mul2(f2 gate, f2 up) {
+  constexpr float kLog2e = 1.44269504f, kLog2eRest = (float)(1.4426950408889634074 - (double)1.44269504f);
+  constexpr float kLn2 = 0.693147181f;
+  const float g0 = lo2(gate), g1 = hi2(gate);
+  const f2 a = pack2(fminf(fabsf(g0), 200.f), fminf(fabsf(g1), 200.f));
+  const f2 t = mul2(a, pack2(kLog2e));
+  f2 rest = fma2(a, pack2(-kLog2e), t);
+  rest = mul2(fma2(a, pack2(-kLog2eRest), rest), pack2(kLn2));
+  f2 e = pack2(ex2(-lo2(t)), ex2(-hi2(t)));
+  e = fma2(e, rest, e);
+  const f2 d = add2(e, pack2(1.f));
+  const f2 minus_y = pack2(rcp(-lo2(d)), rcp(-hi2(d)));
+  const f2 minus_n = mul2(gate, pack2(g0 < 0.f ? -lo2(e) : -1.f, g1 < 0.f ? -hi2(e) : -1.f));
+  const f2 s = mul2(minus_n, minus_y);
+  return mul2(fma2(fma2(s, d, minus_n), minus_y, s), up);
 }
 
 // v / d to nearest for many v and one d: with y the reciprocal of d to nearest and q = v y, the
@@ -223,9 +296,9 @@ __device__ __forceinline__ uint2 encode8x8(const float (&v)[8], int qt) {
 // correctly rounded quotient (P. Markstein, IBM Journal of Research and Development 34(1), 1990) where
 // nothing leaves the range of normal numbers: d is at least 1e-30 here and v at most Q d.  A divisor
 // of infinity or NaN makes the values NaN, as the row's scale says.
-__device__ __forceinline__ float div_by(float v, float d, float y) {
-  const float q = v * y;
-  return fmaf(fmaf(-q, d, v), y, q);
+__device__ __forceinline__ f2 div_by(f2 v, f2 minus_d, f2 y) {
+  const f2 q = mul2(v, y);
+  return fma2(fma2(q, minus_d, v), y, q);
 }
 
 // Whole rows in registers: `warps_per_row` warps share a row, every thread NV groups of eight elements
@@ -256,41 +329,42 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
       if (KIND != FRISK_QUANT_PLAIN && o) ro[i] = load8(o + 8 * (int64_t)gidx);
     }
   }
-  float g[NV][8];
-  float sum = 0.f;
-  uint32_t mx = 0;
+  f2 g[NV][4];
+  f2 sums = 0;      // of squares, even and odd elements
+  float top = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
     if (live && gidx < groups) {
       unpack8(rx[i], g[i]);
+      f2 u[4];
       if (KIND == FRISK_QUANT_SILU_MUL) {
-        float u[8];
         unpack8(ro[i], u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) g[i][j] = silu_mul(g[i][j], u[j]);
+        for (int j = 0; j < 4; ++j) g[i][j] = silu_mul2(g[i][j], u[j]);
       }
       if (KIND == FRISK_QUANT_RMSNORM) {
         if (o) {
-          float u[8];
           unpack8(ro[i], u);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g[i][j] += u[j];
+          for (int j = 0; j < 4; ++j) g[i][j] = add2(g[i][j], u[j]);
           if (so) store8(so + 8 * (int64_t)gidx, g[i]);   // read above by this thread, if it is x or the residual
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(g[i][j], g[i][j], sum);
+        for (int j = 0; j < 4; ++j) sums = fma2(g[i][j], g[i][j], sums);
         if (w) {
-          float u[8];
-          unpack8(load8_shared_by_rows(w + 8 * (int64_t)gidx), u);
+          f2 v[4];
+          unpack8(load8_shared_by_rows(w + 8 * (int64_t)gidx), v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) g[i][j] *= u[j];
+          for (int j = 0; j < 4; ++j) g[i][j] = mul2(g[i][j], v[j]);
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) mx = max(mx, abs_bits(g[i][j]));
+      for (int j = 0; j < 4; ++j) top = abs_max(g[i][j], top);
     }
   }
+  float sum = lo2(sums) + hi2(sums);
+  uint32_t mx = __float_as_uint(top);
   warp_fold<KIND>(sum, mx);
   if (wpr > 1) {
     if (lane == 0) {
@@ -309,16 +383,16 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[i][j] *= 0x1p96f;
+      for (int j = 0; j < 4; ++j) g[i][j] = mul2(g[i][j], pack2(0x1p96f));
   }
-  const float y = __frcp_rn(d);
+  const f2 minus_d = pack2(-d), y = pack2(__frcp_rn(d));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
     if (gidx < groups) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) g[i][j] = div_by(g[i][j], d, y);
+      for (int j = 0; j < 4; ++j) g[i][j] = div_by(g[i][j], minus_d, y);
       *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = encode8x8(g[i], p.q_type);
     }
   }

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional
 
 import numpy as np
@@ -84,11 +85,6 @@ class QuantDesc(C.Structure):
     _fields_ = [("rows", C.c_int64), ("cols", C.c_int64), ("ldx", C.c_int64), ("ldo", C.c_int64), ("lds", C.c_int64),
                 ("ldq", C.c_int64), ("kind", C.c_int32), ("in_type", C.c_int32), ("weight_type", C.c_int32),
                 ("q_type", C.c_int32), ("eps", C.c_float), ("device", C.c_int32)]
-
-
-class QuantArgs(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("up", C.c_void_p),
-                ("sum_out", C.c_void_p), ("q", C.c_void_p), ("scale", C.c_void_p), ("stream", C.c_void_p)]
 
 
 QUANT_KINDS = {"plain": 0, "rmsnorm": 1, "silu_mul": 2}
@@ -201,9 +197,9 @@ def lib() -> C.CDLL:
     L.frisk_b200_reduce_run.restype = C.c_int
     L.frisk_b200_reduce_run_host.argtypes = [C.POINTER(ReduceDesc), vp, vp]
     L.frisk_b200_reduce_run_host.restype = C.c_int
-    L.frisk_b200_quant_run.argtypes = [C.POINTER(QuantDesc), C.POINTER(QuantArgs)]
+    L.frisk_b200_quant_run.argtypes = [C.POINTER(QuantDesc), C.c_char_p]
     L.frisk_b200_quant_run.restype = C.c_int
-    L.frisk_b200_quant_run_host.argtypes = [C.POINTER(QuantDesc), C.POINTER(QuantArgs)]
+    L.frisk_b200_quant_run_host.argtypes = [C.POINTER(QuantDesc), C.c_char_p]
     L.frisk_b200_quant_run_host.restype = C.c_int
     L.frisk_b200_measure_mma_peak.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                               C.POINTER(C.c_double), C.POINTER(C.c_double)]
@@ -228,12 +224,14 @@ def _ptr(x) -> Optional[int]:
     """Device or host address of a torch tensor / numpy array / int / None."""
     if x is None:
         return None
+    try:   # the tensors of a launch first: its cost on the host is of the order of a small kernel
+        return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, int):
         return x
     if isinstance(x, np.ndarray):
         return x.ctypes.data
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
@@ -420,15 +418,20 @@ def quant_desc(rows: int, cols: int, in_type: int, q_type: int, kind: str = "pla
                      in_type if weight_type is None else weight_type, q_type, eps, device)
 
 
-def _quant_args(x, q, scale, weight, residual, up, sum_out, stream) -> QuantArgs:
-    return QuantArgs(_ptr(x), _ptr(residual), _ptr(weight), _ptr(up), _ptr(sum_out), _ptr(q), _ptr(scale), stream)
+_QUANT_ARGS = struct.Struct("8N")   # frisk_quant_args: packing it costs a fraction of filling a ctypes structure
+
+
+def _quant_args(x, q, scale, weight, residual, up, sum_out, stream) -> bytes:
+    return _QUANT_ARGS.pack(_ptr(x) or 0, _ptr(residual) or 0, _ptr(weight) or 0, _ptr(up) or 0, _ptr(sum_out) or 0,
+                            _ptr(q) or 0, _ptr(scale) or 0, stream or 0)
 
 
 def quant_run(desc: QuantDesc, x, q, scale, *, weight=None, residual=None, up=None, sum_out=None,
               stream: int = 0) -> None:
     """Asynchronous launch on device buffers (torch CUDA tensors or raw addresses)."""
-    a = _quant_args(x, q, scale, weight, residual, up, sum_out, stream or None)
-    _check(lib().frisk_b200_quant_run(C.byref(desc), C.byref(a)), "quant_run")
+    rc = (_lib or lib()).frisk_b200_quant_run(C.byref(desc), _quant_args(x, q, scale, weight, residual, up, sum_out, stream))
+    if rc:
+        _check(rc, "quant_run")
 
 
 def quant_host(x: np.ndarray, in_type: int, q_type: int, kind: str = "plain", *, weight: Optional[np.ndarray] = None,
@@ -458,7 +461,7 @@ def quant_host(x: np.ndarray, in_type: int, q_type: int, kind: str = "plain", *,
     scale = np.zeros((rows,), np.float32)
     total = np.zeros((rows, cols), x.dtype) if want_sum else None
     a = _quant_args(x, q, scale, other.get("weight"), other.get("residual"), other.get("up"), total, None)
-    _check(lib().frisk_b200_quant_run_host(C.byref(desc), C.byref(a)), "quant_run_host")
+    _check(lib().frisk_b200_quant_run_host(C.byref(desc), a), "quant_run_host")
     return (q, scale, total) if want_sum else (q, scale)
 
 
