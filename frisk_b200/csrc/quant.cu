@@ -55,45 +55,86 @@ bool rows_on(const void* ptr, int64_t ld, int es, int to) {
 }
 
 constexpr int kMaxGroups = 4;   // groups of eight elements a thread holds at most
+constexpr size_t kRingBytes = 226 * 1024;   // shared memory of a CTA for rows in flight, but for a little
+
+// Opts a kernel into kRingBytes of shared memory, once per device.
+template <typename TIn, bool kFull>
+cudaError_t allow_ring(int device) {
+  static bool done[64] = {};
+  const bool tracked = device >= 0 && device < 64;
+  if (tracked && __atomic_load_n(&done[device], __ATOMIC_ACQUIRE)) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(frisk_quant::quant_gated_stream_kernel<TIn, kMaxGroups, kFull>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+  if (e == cudaSuccess && tracked) __atomic_store_n(&done[device], true, __ATOMIC_RELEASE);
+  return e;
+}
 
 template <typename TIn, typename TW, int KIND>
-cudaError_t launch(Params p, int sms, cudaStream_t st) {
+cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   const int es = sizeof(TIn);
   const bool aligned = p.cols % 8 == 0 && rows_on(p.x, p.ldx, es, 16) && rows_on(p.other, p.ldo, es, 16) &&
                        rows_on(p.sum_out, p.lds, es, 16) && rows_on(p.q, p.ldq, 1, 8) && rows_on(p.weight, 0, 1, 16);
-  const int64_t groups = p.cols / 8;
-  if (!aligned || groups > 1024 * kMaxGroups) {
-    frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND>
-        <<<(unsigned)std::min<int64_t>(p.rows, 0x7fffffff), 256, 0, st>>>(p);
+  constexpr int64_t kMaxCtas = 0x7fffffff;
+  if (p.cols > 8 * 1024 * kMaxGroups || p.rows > kMaxCtas) {   // more than registers hold, or than a grid
+    frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND><<<(unsigned)std::min(p.rows, kMaxCtas), 256, 0, st>>>(p);
     return cudaGetLastError();
   }
-  // Many rows: four groups a thread, the most loads in flight per warp that registers allow; few rows:
-  // one, so that a row is spread over as many threads as there are.
+  const int64_t groups = ceil_div(p.cols, 8);
+  if constexpr (KIND == FRISK_QUANT_SILU_MUL) {
+    // Streamed from two fillings of all SMs' rings on (bf16 / f16, in registers -> streamed: 67 MB of
+    // input 19.2 -> 19.2 us, 98 MB 30.8 -> 27.4, 134 MB 39.1 -> 34.7, 537 MB 73.0 -> 61.6; 33 MB 10.0 ->
+    // 13.0, 39 MB 14.1 -> 14.9).
+    const size_t row = 2 * (size_t)p.cols * es;
+    const int stages = (int)std::min<size_t>(frisk_quant::kMaxRowStages, kRingBytes / row);
+    const int wpr = (int)ceil_div(groups, 32 * kMaxGroups);
+    if (aligned && wpr >= 4 && stages >= 2 && p.rows >= 4 * (int64_t)sms &&
+        (size_t)p.rows * row >= 2 * kRingBytes * sms) {
+      const int teams = std::min(32 / wpr, stages);
+      p.stages = stages;
+      const bool full = p.cols == 256ll * kMaxGroups * wpr;
+      auto kern = full ? frisk_quant::quant_gated_stream_kernel<TIn, kMaxGroups, true>
+                       : frisk_quant::quant_gated_stream_kernel<TIn, kMaxGroups, false>;
+      if (const cudaError_t e = full ? allow_ring<TIn, true>(device) : allow_ring<TIn, false>(device)) return e;
+      kern<<<(unsigned)sms, dim3(32 * wpr, teams), stages * row, st>>>(p);
+      return cudaGetLastError();
+    }
+  }
+  // Many rows: four groups a thread (two without 16-byte accesses), the most loads in flight per warp
+  // that registers allow; few rows: one, so that a row is spread over as many threads as there are.
   const bool few = p.rows < 2 * (int64_t)sms;
-  int nv = few ? 1 : kMaxGroups;
+  int nv = few ? 1 : aligned ? kMaxGroups : 2;
   while (ceil_div(groups, 32 * nv) > 32) nv *= 2;
   while (nv > 1 && 32 * (nv / 2) >= groups) nv /= 2;   // short rows: no more than a warp can use
-  p.warps_per_row = (int)ceil_div(groups, 32 * nv);
-  p.rows_per_cta = std::max(1, 8 / p.warps_per_row);
-  const int64_t ctas = ceil_div(p.rows, p.rows_per_cta);
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  const unsigned threads = 32u * p.warps_per_row * p.rows_per_cta;
+  const int wpr = (int)ceil_div(groups, 32 * nv), rows_per_cta = std::max(1, 8 / wpr);
+  const int64_t ctas = ceil_div(p.rows, rows_per_cta);
+  const dim3 threads(32 * wpr, rows_per_cta);
+  const bool full = p.cols == 256ll * nv * wpr && p.rows % rows_per_cta == 0;
+  auto go = [&](auto kern) { kern<<<(unsigned)ctas, threads, 0, st>>>(p); };
+  using namespace frisk_quant;
+  if (!aligned) {
+    switch (nv) {
+      case 1: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 1>); break;
+      case 2: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 2>); break;
+      default: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 4>); break;
+    }
+    return cudaGetLastError();
+  }
   switch (nv) {
-    case 1: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 1><<<(unsigned)ctas, threads, 0, st>>>(p); break;
-    case 2: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 2><<<(unsigned)ctas, threads, 0, st>>>(p); break;
-    default: frisk_quant::quant_rows_kernel<TIn, TW, KIND, 4><<<(unsigned)ctas, threads, 0, st>>>(p); break;
+    case 1: full ? go(quant_rows_kernel<TIn, TW, KIND, 1, true>) : go(quant_rows_kernel<TIn, TW, KIND, 1, false>); break;
+    case 2: full ? go(quant_rows_kernel<TIn, TW, KIND, 2, true>) : go(quant_rows_kernel<TIn, TW, KIND, 2, false>); break;
+    default: full ? go(quant_rows_kernel<TIn, TW, KIND, 4, true>) : go(quant_rows_kernel<TIn, TW, KIND, 4, false>); break;
   }
   return cudaGetLastError();
 }
 
 template <typename TIn>
-cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, int sms, cudaStream_t st) {
+cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, int device, int sms, cudaStream_t st) {
   switch (d.kind) {
-    case FRISK_QUANT_PLAIN: return launch<TIn, TIn, FRISK_QUANT_PLAIN>(p, sms, st);
-    case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, FRISK_QUANT_SILU_MUL>(p, sms, st);
+    case FRISK_QUANT_PLAIN: return launch<TIn, TIn, FRISK_QUANT_PLAIN>(p, device, sms, st);
+    case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, FRISK_QUANT_SILU_MUL>(p, device, sms, st);
     default:
-      return d.weight_type == d.in_type ? launch<TIn, TIn, FRISK_QUANT_RMSNORM>(p, sms, st)
-                                        : launch<TIn, float, FRISK_QUANT_RMSNORM>(p, sms, st);
+      return d.weight_type == d.in_type ? launch<TIn, TIn, FRISK_QUANT_RMSNORM>(p, device, sms, st)
+                                        : launch<TIn, float, FRISK_QUANT_RMSNORM>(p, device, sms, st);
   }
 }
 
@@ -147,9 +188,9 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) {
     switch (d.in_type) {
-      case FRISK_DT_F32: e = launch_kind<float>(d, p, sms, st); break;
-      case FRISK_DT_F16: e = launch_kind<__half>(d, p, sms, st); break;
-      default: e = launch_kind<__nv_bfloat16>(d, p, sms, st); break;
+      case FRISK_DT_F32: e = launch_kind<float>(d, p, dev, sms, st); break;
+      case FRISK_DT_F16: e = launch_kind<__half>(d, p, dev, sms, st); break;
+      default: e = launch_kind<__nv_bfloat16>(d, p, dev, sms, st); break;
     }
   }
   if (prev >= 0 && prev != d.device) cudaSetDevice(prev);

@@ -21,6 +21,7 @@
 #include <cstdint>
 
 #include "../../include/frisk_b200.h"
+#include "ptx_sm100.cuh"
 
 namespace frisk_quant {
 
@@ -37,7 +38,7 @@ struct Params {
   int64_t ldx, ldo, lds, ldq;
   float eps;
   int32_t q_type;
-  int32_t warps_per_row, rows_per_cta;   // quant_rows_kernel
+  int32_t stages;       // streamed rows: rows in the ring
 };
 
 template <typename T>
@@ -62,8 +63,7 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 __device__ __forceinline__ float q_max(int qt) {
   return qt == FRISK_DT_I8 ? 127.f : qt == FRISK_DT_E4M3 ? 448.f : 57344.f;
 }
-// Values of at most Q in magnitude (a little above it by rounding) into their 8 bits; NaN becomes 0
-// in int8, which has none.
+// A finite value of at most Q in magnitude (a little above it by rounding) into its 8 bits.
 __device__ __forceinline__ uint8_t encode8(float v, int qt) {
   if (qt == FRISK_DT_I8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(v)));
   return (uint8_t)__nv_cvt_float_to_fp8(v, __NV_SATFINITE, qt == FRISK_DT_E4M3 ? __NV_E4M3 : __NV_E5M2);
@@ -148,11 +148,13 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       mx = max(mx, s_max[i]);
     }
     const float divisor = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
+    const bool finite = divisor <= 3.402823466e38f;
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
     // sum_out may be x or the residual: an element is written by the thread that has just read it
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
-      q[c] = encode8(__fdiv_rn(value(c, &h), divisor), p.q_type);
+      const float v = value(c, &h);
+      q[c] = finite ? encode8(__fdiv_rn(v, divisor), p.q_type) : 0;
       if (KIND == FRISK_QUANT_RMSNORM && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
@@ -232,6 +234,12 @@ __device__ __forceinline__ void unpack8(const Eight<T>& r, f2 (&f)[4]) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) f[j] = pack2(to_float<T>(e[2 * j]), to_float<T>(e[2 * j + 1]));
 }
+template <>
+__device__ __forceinline__ void unpack8<__nv_bfloat16>(const Eight<__nv_bfloat16>& r, f2 (&f)[4]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};   // a bf16 is the upper half of its fp32
+#pragma unroll
+  for (int j = 0; j < 4; ++j) f[j] = pack2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const f2 (&f)[4]) {
   Eight<T> r;
@@ -251,13 +259,18 @@ __device__ __forceinline__ uint2 encode8x8(const f2 (&v)[4], int qt) {
     uint16_t h[4];
   } r;
   if (qt == FRISK_DT_I8) {
-    // (|v| rounds to 127 at most; NaN becomes 0)
+    // v + 1.5 * 2^23 rounds v to the nearest integer, ties to even, and holds it in its low byte
+    // (the conversion instruction shares its unit with the gate's 2^x and reciprocal)
+    uint32_t b[8];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t upper;
-      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(upper) : "r"(__float2int_rn(hi2(v[2 * j + 1]))), "r"(__float2int_rn(lo2(v[2 * j + 1]))), "r"(0));
-      asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(r.u[j]) : "r"(__float2int_rn(hi2(v[2 * j]))), "r"(__float2int_rn(lo2(v[2 * j]))), "r"(upper));
+    for (int j = 0; j < 4; ++j) {
+      const f2 m = add2(v[j], pack2(12582912.f));
+      b[2 * j] = __float_as_uint(lo2(m));
+      b[2 * j + 1] = __float_as_uint(hi2(m));
     }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      r.u[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
   } else if (qt == FRISK_DT_E4M3) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[j]), hi2(v[j])), __NV_SATFINITE, __NV_E4M3);
@@ -268,53 +281,120 @@ __device__ __forceinline__ uint2 encode8x8(const f2 (&v)[4], int qt) {
   return make_uint2(r.u[0], r.u[1]);
 }
 
-// gate / (1 + exp(-gate)) * up for two elements.  With e = exp(-|gate|), which cannot overflow:
-//   silu = gate * (gate < 0 ? e : 1) / (1 + e).
-// e = 2^-(a log2(e)), a = |gate| (at most 200: e is 0 long before): the product is split into its
-// rounded value t, for the hardware's 2^x, and the exact rest, which with log2(e)'s own rest enters
-// to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's, corrected by its remainder
-// as in div_by.  Exponentials below 2^-126 (gates below -87) are zero.
+// gate / (1 + exp(-gate)) * up for two elements.  e = exp(-gate) = 2^t, t = -gate log2(e): the product
+// is split into its rounded value, for the hardware's 2^x, and the exact rest, which with log2(e)'s own
+// rest enters to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's, corrected by
+// its remainder as in div_by.  The exponent is taken of gates held to [-88, 200]: above, e is zero
+// already; at -88 the reciprocal of 1 + e is below 2^-126, which the hardware flushes to zero, so
+// gates below -87.3 give zero (gate = NaN still enters as the dividend).
 __device__ __forceinline__ f2 silu_mul2(f2 gate, f2 up) {
   constexpr float kLog2e = 1.44269504f, kLog2eRest = (float)(1.4426950408889634074 - (double)1.44269504f);
   constexpr float kLn2 = 0.693147181f;
-  const float g0 = lo2(gate), g1 = hi2(gate);
-  const f2 a = pack2(fminf(fabsf(g0), 200.f), fminf(fabsf(g1), 200.f));
+  const f2 a = pack2(fminf(fmaxf(lo2(gate), -88.f), 200.f), fminf(fmaxf(hi2(gate), -88.f), 200.f));
   const f2 t = mul2(a, pack2(kLog2e));
   f2 rest = fma2(a, pack2(-kLog2e), t);
   rest = mul2(fma2(a, pack2(-kLog2eRest), rest), pack2(kLn2));
   f2 e = pack2(ex2(-lo2(t)), ex2(-hi2(t)));
   e = fma2(e, rest, e);
-  const f2 d = add2(e, pack2(1.f));
-  const f2 minus_y = pack2(rcp(-lo2(d)), rcp(-hi2(d)));
-  const f2 minus_n = mul2(gate, pack2(g0 < 0.f ? -lo2(e) : -1.f, g1 < 0.f ? -hi2(e) : -1.f));
-  const f2 s = mul2(minus_n, minus_y);
-  return mul2(fma2(fma2(s, d, minus_n), minus_y, s), up);
+  const f2 minus_d = fma2(e, pack2(-1.f), pack2(-1.f));
+  const f2 y = pack2(rcp(-lo2(minus_d)), rcp(-hi2(minus_d)));
+  const f2 s = mul2(gate, y);
+  return mul2(fma2(fma2(s, minus_d, gate), y, s), up);
 }
 
 // v / d to nearest for many v and one d: with y the reciprocal of d to nearest and q = v y, the
 // remainder v - q d is exact in one fused multiply-add, and q plus the remainder times y is the
 // correctly rounded quotient (P. Markstein, IBM Journal of Research and Development 34(1), 1990) where
-// nothing leaves the range of normal numbers: d is at least 1e-30 here and v at most Q d.  A divisor
-// of infinity or NaN makes the values NaN, as the row's scale says.
+// nothing leaves the range of normal numbers: d is at least 1e-30 and finite here, and v at most Q d.
 __device__ __forceinline__ f2 div_by(f2 v, f2 minus_d, f2 y) {
   const f2 q = mul2(v, y);
   return fma2(fma2(q, minus_d, v), y, q);
 }
 
-// Whole rows in registers: `warps_per_row` warps share a row, every thread NV groups of eight elements
-// of it, so the row is read once and the only pause is the fold of (sum, maximum) over the warps.
+// Eight elements from storage to g, with the running sum of squares and maximum.  `weights(v)` fills v
+// with the elements' weights, false if there are none; `store_sum(h)` stores h where that is wanted (x
+// and the residual have been read: it may go to either).
+template <typename TIn, int KIND, typename Weights, typename StoreSum>
+__device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TIn>& other, bool has_other, Weights weights,
+                                             StoreSum store_sum, f2 (&g)[4], f2& sums, float& top) {
+  unpack8(x, g);
+  f2 u[4];
+  if (KIND == FRISK_QUANT_SILU_MUL) {
+    unpack8(other, u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = silu_mul2(g[j], u[j]);
+  }
+  if (KIND == FRISK_QUANT_RMSNORM) {
+    if (has_other) {
+      unpack8(other, u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = add2(g[j], u[j]);
+      store_sum(g);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums = fma2(g[j], g[j], sums);
+    f2 v[4];
+    if (weights(v)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = mul2(g[j], v[j]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) top = abs_max(g[j], top);
+}
+
+// g over the divisor, in place.
+template <int NV>
+__device__ __forceinline__ void divide(f2 (&g)[NV][4], float d) {
+  if (!(d >= 1e-30f && d <= 3.402823466e38f)) {
+    // a small divisor: both up by the same power of two (exact), so that div_by stays in range; a
+    // divisor of infinity or NaN: zeros, next to a scale that makes every product NaN
+    const bool small = d < 1.f;
+    d = small ? d * 0x1p96f : 1.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[i][j] = small ? mul2(g[i][j], pack2(0x1p96f)) : 0;
+  }
+  const f2 minus_d = pack2(-d), y = pack2(__frcp_rn(d));
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[i][j] = div_by(g[i][j], minus_d, y);
+}
+
+// Sum and maximum over the `wpr` warps of each of the CTA's rows, in every thread (a CTA barrier).
+template <int KIND>
+__device__ __forceinline__ void row_fold(float& sum, uint32_t& mx, float* s_sum, uint32_t* s_max, int warp, int lane,
+                                         int slot, int wpr) {
+  warp_fold<KIND>(sum, mx);
+  if (wpr == 1) return;
+  if (lane == 0) {
+    s_sum[warp] = sum;
+    s_max[warp] = mx;
+  }
+  __syncthreads();
+  sum = lane < wpr ? s_sum[slot * wpr + lane] : 0.f;
+  mx = lane < wpr ? s_max[slot * wpr + lane] : 0u;
+  warp_fold<KIND>(sum, mx);
+}
+
+// Whole rows in registers: blockDim.x threads (whole warps) share a row, each with NV groups of eight
+// elements of it, so the row is read once and the only pause is the fold of (sum, maximum) over the
+// warps.
 // For rows whose starts, in every buffer, allow 16-byte accesses (8 for q) and whose width is a
-// multiple of eight.  CTAs of more than one row fold them side by side.
-template <typename TIn, typename TW, int KIND, int NV>
+// multiple of eight.  CTAs of more than one row (blockDim.y) fold them side by side.
+// kFull: every thread has all of its groups, of a row that exists (no bounds to test).
+template <typename TIn, typename TW, int KIND, int NV, bool kFull>
 __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wpr = p.warps_per_row;
-  const int slot = warp / wpr, warp_in_row = warp - slot * wpr;
-  const int64_t r = (int64_t)blockIdx.x * p.rows_per_cta + slot;
-  const bool live = r < p.rows;
-  const int t = warp_in_row * 32 + lane, step = wpr * 32, groups = (int)(p.cols >> 3);
+  // threadIdx.y: which of the CTA's rows (the same in a whole warp: the broadcast tells the compiler)
+  const int t = threadIdx.x, step = blockDim.x, lane = t & 31, wpr = step >> 5;
+  const int slot = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp = slot * wpr + (t >> 5);
+  const int64_t r = (int64_t)blockIdx.x * blockDim.y + slot;
+  const bool live = kFull || r < p.rows;
+  const int groups = (int)(p.cols >> 3);
   const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
   const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
   const TW* w = static_cast<const TW*>(p.weight);
@@ -324,7 +404,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
-    if (live && gidx < groups) {
+    if (kFull || (live && gidx < groups)) {
       rx[i] = load8(x + 8 * (int64_t)gidx);
       if (KIND != FRISK_QUANT_PLAIN && o) ro[i] = load8(o + 8 * (int64_t)gidx);
     }
@@ -335,65 +415,247 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
-    if (live && gidx < groups) {
-      unpack8(rx[i], g[i]);
-      f2 u[4];
-      if (KIND == FRISK_QUANT_SILU_MUL) {
-        unpack8(ro[i], u);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) g[i][j] = silu_mul2(g[i][j], u[j]);
-      }
-      if (KIND == FRISK_QUANT_RMSNORM) {
-        if (o) {
-          unpack8(ro[i], u);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) g[i][j] = add2(g[i][j], u[j]);
-          if (so) store8(so + 8 * (int64_t)gidx, g[i]);   // read above by this thread, if it is x or the residual
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sums = fma2(g[i][j], g[i][j], sums);
-        if (w) {
-          f2 v[4];
-          unpack8(load8_shared_by_rows(w + 8 * (int64_t)gidx), v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) g[i][j] = mul2(g[i][j], v[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = abs_max(g[i][j], top);
-    }
+    if (kFull || (live && gidx < groups))
+      group_values<TIn, KIND>(
+          rx[i], ro[i], o != nullptr,
+          [&](f2 (&v)[4]) {
+            if (w) unpack8(load8_shared_by_rows(w + 8 * gidx), v);
+            return w != nullptr;
+          },
+          [&](const f2 (&h)[4]) {
+            if (so) store8(so + 8 * (int64_t)gidx, h);
+          },
+          g[i], sums, top);
   }
   float sum = lo2(sums) + hi2(sums);
   uint32_t mx = __float_as_uint(top);
-  warp_fold<KIND>(sum, mx);
-  if (wpr > 1) {
-    if (lane == 0) {
-      s_sum[warp] = sum;
-      s_max[warp] = mx;
-    }
-    __syncthreads();
-    sum = lane < wpr ? s_sum[slot * wpr + lane] : 0.f;
-    mx = lane < wpr ? s_max[slot * wpr + lane] : 0u;
-    warp_fold<KIND>(sum, mx);
-  }
+  row_fold<KIND>(sum, mx, s_sum, s_max, warp, lane, slot, wpr);
   if (!live) return;
-  float d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
-  if (d < 1e-30f) {   // both up by the same power of two (exact), so that div_by stays in range
-    d *= 0x1p96f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) g[i][j] = mul2(g[i][j], pack2(0x1p96f));
-  }
-  const f2 minus_d = pack2(-d), y = pack2(__frcp_rn(d));
+  divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
-    if (gidx < groups) {
+    if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = encode8x8(g[i], p.q_type);
+  }
+}
+
+// The same for rows at any alignment and width: the threads of a row take neighbouring ELEMENTS, the
+// e-th of a thread lying e x (threads per row) further on, so that every access of a warp is one run
+// of 32 elements.  Elements past the end of the row are zeros.
+template <typename TIn, typename TW, int KIND, int NV>
+__global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params p) {
+  __shared__ float s_sum[32];
+  __shared__ uint32_t s_max[32];
+  constexpr int NE = 8 * NV;
+  const int t = threadIdx.x, step = blockDim.x, lane = t & 31, wpr = step >> 5;
+  const int slot = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp = slot * wpr + (t >> 5);
+  const int64_t r = (int64_t)blockIdx.x * blockDim.y + slot;
+  const int left = r < p.rows ? (int)p.cols - t : 0;   // element e exists where e * step < left
+  const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
+  const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
+  const TW* w = static_cast<const TW*>(p.weight);
+  TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
+  uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+  auto at = [&](int e) { return (uint32_t)(t + e * step); };
+
+  TIn rx[NE], ro[NE];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[i][j] = div_by(g[i][j], minus_d, y);
-      *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = encode8x8(g[i], p.q_type);
+  for (int e = 0; e < NE; ++e) {
+    rx[e] = ro[e] = from_float<TIn>(0.f);
+    if (e * step < left) rx[e] = x[at(e)];
+  }
+  if (KIND != FRISK_QUANT_PLAIN && o) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+      if (e * step < left) ro[e] = o[at(e)];
+  }
+  f2 g[NV][4];
+  f2 sums = 0;
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int e = 8 * i + 2 * j;
+      f2 v = pack2(to_float<TIn>(rx[e]), to_float<TIn>(rx[e + 1]));
+      const f2 u = pack2(to_float<TIn>(ro[e]), to_float<TIn>(ro[e + 1]));
+      if (KIND == FRISK_QUANT_SILU_MUL) v = silu_mul2(v, u);
+      if (KIND == FRISK_QUANT_RMSNORM) {
+        v = add2(v, u);   // (x and the residual have been read: h may go to either)
+        sums = fma2(v, v, sums);
+        if (so) {
+          if (e * step < left) so[at(e)] = from_float<TIn>(lo2(v));
+          if ((e + 1) * step < left) so[at(e + 1)] = from_float<TIn>(hi2(v));
+        }
+        if (w) {
+          TW w0 = from_float<TW>(0.f), w1 = w0;
+          if (e * step < left) w0 = w[at(e)];
+          if ((e + 1) * step < left) w1 = w[at(e + 1)];
+          v = mul2(v, pack2(to_float<TW>(w0), to_float<TW>(w1)));
+        }
+      }
+      top = abs_max(v, top);
+      g[i][j] = v;
+    }
+  float sum = lo2(sums) + hi2(sums);
+  uint32_t mx = __float_as_uint(top);
+  row_fold<KIND>(sum, mx, s_sum, s_max, warp, lane, slot, wpr);
+  if (r >= p.rows) return;
+  divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const uint2 b = encode8x8(g[i], p.q_type);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if ((8 * i + k) * step < left) q[at(8 * i + k)] = (uint8_t)((k < 4 ? b.x : b.y) >> (8 * (k & 3)));
+  }
+}
+
+// ---- many gated rows: streamed through shared memory ---------------------------------------------
+// The gate costs enough arithmetic that rows in registers alternate between loading and computing
+// (4096 x 16384 bf16: 73 us at half the DRAM rate and 54 % of the issue slots; streamed 62 us; the
+// other kinds are faster in registers: norm 8192 x 8192 with residual 79 against 80 us, fp32 8192 x
+// 8192 as it is 50 against 55).
+// One CTA per SM walks the rows blockIdx.x, + gridDim.x, ...; bulk copies bring them into a ring of
+// `stages` whole rows (both operands), several ahead of the arithmetic, so that the memory is read
+// without a pause while rows are folded, divided and stored.  The CTA is blockDim.y teams of
+// blockDim.x threads; a team takes every blockDim.y-th row, so that one team's barrier is another's
+// arithmetic.  The row's stage is refilled as soon as its team has read it into registers.
+// Waits are bounded: a team whose copies do not arrive gives up and leaves NaN in its rows' scales.
+constexpr int kMaxRowStages = 16;
+constexpr long long kRowWaitCycles = 1ll << 29;   // about 0.3 s
+
+__device__ __forceinline__ uint32_t load_tag(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.acquire.cta.shared::cta.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_tag(uint32_t addr, uint32_t v) {
+  asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+// Waits for row `row` of this CTA in the stage behind `bar`.  A phase's parity alone does not say
+// which row it is: a team may be ahead of the one that has yet to read the stage's row before, and
+// would take the phase before that for its own.  So the stage's tag, set when a row is asked for,
+// comes first; from then on the barrier is in that row's phase or past it.
+__device__ __forceinline__ bool wait_row(uint32_t bar, uint32_t parity, uint32_t tag, uint32_t row) {
+  if (load_tag(tag) == row && frisk::ptx::mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (clock64() - t0 < kRowWaitCycles)
+    if (load_tag(tag) == row && frisk::ptx::mbar_try_wait(bar, parity)) return true;
+  return false;
+}
+// Barrier of one team (hardware barrier 1 + team): true if any thread brings `bad`.
+__device__ __forceinline__ bool team_barrier(int team, int threads, bool bad) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}"
+      : "=r"(any)
+      : "r"(1 + team), "r"(threads), "r"((uint32_t)bad)
+      : "memory");
+  return any != 0;
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> load8_smem(uint32_t addr) {
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w[i].x), "=r"(r.w[i].y), "=r"(r.w[i].z), "=r"(r.w[i].w)
+                 : "r"(addr + 16 * i)
+                 : "memory");
+  return r;
+}
+
+template <typename TIn, int NV, bool kFull>
+__global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Params p) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[kMaxRowStages];
+  __shared__ uint32_t tags[kMaxRowStages];   // which of the CTA's rows a stage was last asked for
+  __shared__ uint32_t s_max[2][32];
+  const int t = threadIdx.x, step = blockDim.x, lane = t & 31, wpr = step >> 5;
+  const int teams = blockDim.y, stages = p.stages;
+  const int team = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp = team * wpr + (t >> 5);
+  const int groups = (int)(p.cols >> 3);
+  const uint32_t bytes = (uint32_t)p.cols * (uint32_t)sizeof(TIn);   // of one operand's row
+  const uint32_t stage_bytes = 2 * bytes;
+  const uint32_t ring0 = frisk::ptx::smem_u32(ring), bar0 = frisk::ptx::smem_u32(bars);
+  const uint32_t tag0 = frisk::ptx::smem_u32(tags);
+  const int64_t n = (p.rows - blockIdx.x + gridDim.x - 1) / gridDim.x;   // rows of this CTA
+
+  auto fetch = [&](int64_t j, int stage) {   // one thread: row j of this CTA into a stage
+    const int64_t r = blockIdx.x + j * gridDim.x;
+    const uint32_t dst = ring0 + stage * stage_bytes, bar = bar0 + 8 * stage;
+    store_tag(tag0 + 4 * stage, (uint32_t)j);
+    frisk::ptx::mbar_arrive_expect_tx(bar, stage_bytes);
+    frisk::ptx::bulk_load(dst, static_cast<const TIn*>(p.x) + r * p.ldx, bytes, bar);
+    frisk::ptx::bulk_load(dst + bytes, static_cast<const TIn*>(p.other) + r * p.ldo, bytes, bar);
+  };
+  if (threadIdx.x == 0 && threadIdx.y == 0) {
+    for (int s = 0; s < stages; ++s) {
+      frisk::ptx::mbar_init(bar0 + 8 * s, 1);
+      tags[s] = 0xffffffffu;   // (n is below that: checked when launching)
+    }
+    frisk::ptx::fence_mbar_init();
+    for (int s = 0; s < stages && s < n; ++s) fetch(s, s);
+  }
+  __syncthreads();
+
+  int stage = team;
+  uint32_t phase = 0;
+  int buf = 0;
+  for (int64_t j = team; j < n; j += teams) {   // teams <= stages
+    const int64_t r = blockIdx.x + j * gridDim.x;
+    const bool ok = wait_row(bar0 + 8 * stage, phase, tag0 + 4 * stage, (uint32_t)j);
+    const uint32_t at = ring0 + stage * stage_bytes;
+    f2 g[NV][4];
+    f2 sums = 0;
+    float top = 0.f;
+    if (ok) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int gidx = t + i * step;
+        if (kFull || gidx < groups) {
+          const uint32_t e = at + (uint32_t)gidx * 8u * (uint32_t)sizeof(TIn);
+          group_values<TIn, FRISK_QUANT_SILU_MUL>(load8_smem<TIn>(e), load8_smem<TIn>(e + bytes), true,
+                                                  [](f2 (&)[4]) { return false; }, [](const f2 (&)[4]) {}, g[i], sums, top);
+        }
+      }
+    }
+    float sum = 0.f;   // (of the norm)
+    uint32_t mx = __float_as_uint(top);
+    warp_fold<FRISK_QUANT_SILU_MUL>(sum, mx);
+    if (lane == 0) s_max[buf][warp] = mx;
+    if (team_barrier(team, step, !ok)) {
+      if (t == 0) {
+        const long long t0 = clock64();   // copies in flight land before the CTA may leave
+        while (clock64() - t0 < 100000ll) {
+        }
+        for (; j < n; j += teams) p.scale[blockIdx.x + j * gridDim.x] = __uint_as_float(0x7fc00000u);
+      }
+      break;
+    }
+    // every thread of the team has read the stage
+    if (t == 0 && j + stages < n) fetch(j + stages, stage);
+    mx = lane < wpr ? s_max[buf][team * wpr + lane] : 0u;
+    warp_fold<FRISK_QUANT_SILU_MUL>(sum, mx);
+    divide<NV>(g, row_divisor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+    uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int gidx = t + i * step;
+      if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * gidx) = encode8x8(g[i], p.q_type);
+    }
+    buf ^= 1;
+    stage += teams;
+    if (stage >= stages) {
+      stage -= stages;
+      phase ^= 1u;
     }
   }
 }

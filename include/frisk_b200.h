@@ -362,8 +362,7 @@ int frisk_b200_reduce_run_host(const frisk_reduce_desc* desc, const void* src, v
  * with Q = 127 (i8: -128 is not used), 448 (e4m3), 57344 (e5m2).  Arithmetic in fp32 (the norm is of
  * the unrounded h; squares are summed in fp32, so the rows' norms have to stay below 1e19), one
  * rounding into q and one into sum_out.  A row with an infinity or NaN in v, or with squares that
- * overflow, gets a scale of infinity or NaN; its q are 0 or NaN (i8 has no NaN: 0), and every product
- * with its scale is NaN.  A row of zeros gets q = 0 and the scale 2^-126.  The order of the sum is
+ * overflow, gets a scale of infinity or NaN and zeros for q: every product with its scale is NaN.  A row of zeros gets q = 0 and the scale 2^-126.  The order of the sum is
  * fixed by the shape, the types and the alignment.
  */
 typedef enum {

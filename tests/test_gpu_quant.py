@@ -133,7 +133,7 @@ def test_rows_of_zeros_tiny_rows_and_rows_that_are_not_finite(kind, cols, q_type
     assert (np.abs(got[2] - v[2]) <= np.maximum(s[2] * 0.5, np.abs(v[2]) * 2.0 ** -2) + 2.0 ** -140).all()
     assert not got[0].any()
     for r in (4, 5, 6):
-        assert not np.isfinite(s[r]), r
+        assert not np.isfinite(s[r]) and not q[r].any(), r
 
 
 def test_squares_past_fp32_give_no_silent_scale():
@@ -254,3 +254,44 @@ def test_captured_into_a_graph_and_on_another_stream():
         torch.cuda.synchronize()
         v, _ = ref.ref_quant(host, W.BF16, "silu_mul")
         check_q(q.cpu().numpy(), s.cpu().numpy(), v, "silu_mul", W.I8)
+
+
+@pytest.mark.parametrize("q_type", [W.I8, W.E4M3], ids=ids)
+@pytest.mark.parametrize("rows,cols,in_type", [(600, 3080, W.BF16), (1500, 4096, W.F32), (1201, 3336, W.F16), (640, 8192, W.BF16),
+                                               (601, 16384, W.F32), (700, 16384, W.BF16)],
+                         ids=["600x3080", "1500x4096", "1201x3336", "640x8192", "601x16384", "700x16384"])
+@pytest.mark.parametrize("kind", ["plain", "rmsnorm", "silu_mul"])
+def test_many_wide_rows(kind, rows, cols, in_type, q_type):
+    many_rows(kind, rows, cols, in_type, q_type)
+
+
+@pytest.mark.parametrize("rows,cols,in_type,q_type", [(1100, 16384, W.BF16, W.E4M3), (1500, 12008, W.F16, W.I8), (1101, 8192, W.F32, W.E5M2),
+                                                      (4500, 4096, W.BF16, W.I8)],
+                         ids=["1100x16384", "1500x12008", "1101x8192", "4500x4096"])
+def test_gated_rows_streamed_through_shared_memory(rows, cols, in_type, q_type):
+    many_rows("silu_mul", rows, cols, in_type, q_type)
+
+
+def many_rows(kind, rows, cols, in_type, q_type):
+    """More rows than the device holds at once, run three times: the same bits each time."""
+    import torch
+    dev = torch.device("cuda:0")
+    x, kw = inputs(rows, cols, in_type, kind, 12)
+    kw.pop("weight_type", None)
+    on = lambda a: torch.from_numpy(np.ascontiguousarray(a).view(np.uint8)).to(dev)  # noqa: E731
+    bx, extra = on(x), {n: on(a) for n, a in kw.items()}
+    runs = []
+    for _ in range(3):
+        q = torch.zeros((rows, cols), dtype=torch.uint8, device=dev)
+        s = torch.zeros(rows, device=dev)
+        h = torch.zeros((rows, cols * W.ELEM_SIZE[in_type]), dtype=torch.uint8, device=dev) if kind == "rmsnorm" else None
+        R.quant_run(R.quant_desc(rows, cols, in_type, q_type, kind), bx, q, s, sum_out=h, **extra)
+        runs.append((q, s, h))
+    torch.cuda.synchronize()
+    for q, s, h in runs[1:]:
+        assert torch.equal(q, runs[0][0]) and torch.equal(s, runs[0][1]) and (h is None or torch.equal(h, runs[0][2]))
+    v, hw = ref.ref_quant(x, in_type, kind, **kw)
+    q, s, h = runs[0]
+    check_q(q.cpu().numpy().view(W.storage_numpy_dtype(q_type)), s.cpu().numpy(), v, kind, q_type)
+    if kind == "rmsnorm":
+        check_sum(h.cpu().numpy().view(x.dtype), hw, in_type)
