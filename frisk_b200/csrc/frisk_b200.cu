@@ -872,48 +872,92 @@ int launch_finalize_t(const frisk_gemm_plan* pl, float* ws, void* C, const float
   return FRISK_OK;
 }
 
-// Copies `rows` rows of `row_bytes` bytes from pitch `src_pitch` to pitch `dst_pitch` (a multiple
-// of 16, like dst itself), zero behind the end of a row.  The source may start anywhere: it is
-// read in 2-byte or 1-byte units (`unit`), the destination written 16 bytes at a time.
-__global__ void __launch_bounds__(256) repack_rows_kernel(const unsigned char* __restrict__ src,
-                                                          unsigned char* __restrict__ dst, int64_t rows,
-                                                          int64_t row_bytes, int64_t src_pitch,
-                                                          int64_t dst_pitch, int unit) {
-  const int64_t chunks = dst_pitch >> 4;
-  const int64_t total = rows * chunks;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / chunks, c = (i - r * chunks) << 4;
-    const unsigned char* s = src + r * src_pitch + c;
-    union {
-      uint4 v;
-      unsigned short h[8];
-      unsigned char b[16];
-    } u;
-    u.v = make_uint4(0, 0, 0, 0);
-    const int64_t left = row_bytes - c;
-    if (left >= 16 && (reinterpret_cast<uintptr_t>(s) & 15) == 0) {
-      u.v = *reinterpret_cast<const uint4*>(s);
-    } else if (unit == 2) {
+// Rows copied to a pitch that is a multiple of 16 bytes (like dst itself), zero behind the end of a
+// row.  The source may start anywhere and have any pitch.
+struct RepackJob {
+  const unsigned char* src;
+  unsigned char* dst;
+  int64_t rows, row_bytes, src_pitch, dst_pitch;
+  uint32_t segs;   // pieces of kRepackSeg bytes per row
+};
+constexpr int kRepackSeg = 2048;   // a warp's piece: four 16-byte chunks per lane
+
+// Both operands of a gemm in one launch (jobs without rows are empty); a warp per piece of a row.
+// Sixteen bytes of the destination come out of five aligned words of the source, shifted together;
+// only pieces at the ends of a row or of the buffer go byte by byte, so that nothing outside the
+// buffer is read.
+__global__ void __launch_bounds__(256) repack_rows_kernel(const RepackJob a, const RepackJob b) {
+  frisk::ptx::griddep_launch_dependents();
+  frisk::ptx::griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t items_a = a.rows * a.segs, items = items_a + b.rows * b.segs;
+  for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
+    const RepackJob& j = it < items_a ? a : b;
+    const int64_t k = it < items_a ? it : it - items_a;
+    const int64_t r = j.segs == 1 ? k : k / j.segs;
+    const int64_t c0 = (k - r * j.segs) * kRepackSeg;
+    const unsigned char* end = j.src + (j.rows - 1) * j.src_pitch + j.row_bytes;   // of the buffer
+    uint4 v[kRepackSeg / 512];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (2 * j < left) u.h[j] = *reinterpret_cast<const unsigned short*>(s + 2 * j);
-    } else {
+    for (int u = 0; u < kRepackSeg / 512; ++u) {
+      const int64_t c = c0 + (u * 32 + lane) * 16;
+      v[u] = make_uint4(0, 0, 0, 0);
+      if (c >= j.row_bytes) continue;
+      const unsigned char* p = j.src + r * j.src_pitch + c;
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
+      const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3) * 8u;
+      const bool whole = j.row_bytes - c >= 16;
+      if (whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        v[u] = *reinterpret_cast<const uint4*>(p);
+      } else if (whole && reinterpret_cast<const unsigned char*>(w) >= j.src &&
+                 reinterpret_cast<const unsigned char*>(w + 5) <= end) {
+        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4];
+        v[u].x = __funnelshift_r(w0, w1, sh);
+        v[u].y = __funnelshift_r(w1, w2, sh);
+        v[u].z = __funnelshift_r(w2, w3, sh);
+        v[u].w = __funnelshift_r(w3, w4, sh);
+      } else {
+        const int n = (int)(whole ? 16 : j.row_bytes - c);
+        uint32_t x[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < left) u.b[j] = s[j];
+        for (int e = 0; e < 16; ++e)
+          if (e < n) x[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
+        v[u] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
     }
-    *reinterpret_cast<uint4*>(dst + r * dst_pitch + c) = u.v;
+#pragma unroll
+    for (int u = 0; u < kRepackSeg / 512; ++u) {
+      const int64_t c = c0 + (u * 32 + lane) * 16;
+      if (c < j.dst_pitch) *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = v[u];
+    }
   }
 }
 
-int launch_repack(const void* src, void* dst, int64_t rows, int64_t cols, int64_t ld_src, int64_t ld_dst,
-                  int es, int sm_count, cudaStream_t st) {
-  const int64_t work = rows * (ld_dst * es / 16);
-  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>((work + 255) / 256, 8 * (int64_t)sm_count));
-  repack_rows_kernel<<<blocks, 256, 0, st>>>(static_cast<const unsigned char*>(src), static_cast<unsigned char*>(dst),
-                                             rows, cols * es, ld_src * es, ld_dst * es, es);
-  FRISK_CUDA(cudaGetLastError());
+RepackJob repack_job(const void* src, void* dst, int64_t rows, int64_t cols, int64_t ld_src, int64_t ld_dst, int es) {
+  RepackJob j;
+  j.src = static_cast<const unsigned char*>(src);
+  j.dst = static_cast<unsigned char*>(dst);
+  j.rows = rows;
+  j.row_bytes = cols * es;
+  j.src_pitch = ld_src * es;
+  j.dst_pitch = ld_dst * es;
+  j.segs = (uint32_t)((j.dst_pitch + kRepackSeg - 1) / kRepackSeg);
+  return j;
+}
+
+int launch_repack(const RepackJob& a, const RepackJob& b, int sm_count, cudaStream_t st) {
+  const int64_t items = a.rows * a.segs + b.rows * b.segs;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 7) / 8, 8 * (int64_t)sm_count)), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FRISK_CUDA(cudaLaunchKernelEx(&cfg, repack_rows_kernel, a, b));
   return FRISK_OK;
 }
 
@@ -1135,7 +1179,9 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
   // pitch before every run (one more launch each; the copy reads and writes the operand once,
   // against a CUDA-core kernel about 100 x slower on the whole problem).
   if (tcgen05_ineligible_reason(d) == FRISK_TC_PITCH && d.force_kernel != 1 + FRISK_KERNEL_SIMT) {
-    const int64_t es = elem_size(d.a_type), q = 16 / es;
+    // (integers to whole 128-byte lines: rows that start off them cost the tile loads a third of their
+    // rate -- 333 x 1000 x 4112 at a pitch of 4112 bytes 15.6 us, at 4224 11.6 us)
+    const int64_t es = elem_size(d.a_type), q = (d.a_type == FRISK_DT_I8 ? 128 : 16) / es;
     frisk_gemm_desc& k = pl->kd;
     if ((d.lda * es) % 16) {
       k.lda = ((d.transA ? d.M : d.K) + q - 1) / q * q;
@@ -1326,7 +1372,8 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
     pl->kd = pl->d;
   }
   pl->ws_bytes += pl->repack_a_bytes + pl->repack_b_bytes;
-  pl->info.launches += (pl->repack_a_bytes ? 1 : 0) + (pl->repack_b_bytes ? 1 : 0);
+  const int repacked = (pl->repack_a_bytes ? 1 : 0) + (pl->repack_b_bytes ? 1 : 0);
+  pl->info.launches += pl->d.a_type == FRISK_DT_I8 ? std::min(repacked, 1) : repacked;
   *out = pl;
   return FRISK_OK;
 }
@@ -1448,18 +1495,22 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
     if ((uintptr_t)workspace % 16) return FRISK_ERR_MISALIGNED;
     const int es = elem_size(d.a_type);
     char* w = static_cast<char*>(workspace);
+    RepackJob ja{}, jb{};
     if (pl->repack_a_bytes) {
-      if (int rc = launch_repack(A, w, d.transA ? d.K : d.M, d.transA ? d.M : d.K, d.lda, k.lda, es,
-                                 pl->sm_count, st))
-        return rc;
+      ja = repack_job(A, w, d.transA ? d.K : d.M, d.transA ? d.M : d.K, d.lda, k.lda, es);
       A = w;
     }
     if (pl->repack_b_bytes) {
       char* wb = w + pl->repack_a_bytes;
-      if (int rc = launch_repack(B, wb, d.transB ? d.N : d.K, d.transB ? d.K : d.N, d.ldb, k.ldb, es,
-                                 pl->sm_count, st))
-        return rc;
+      jb = repack_job(B, wb, d.transB ? d.N : d.K, d.transB ? d.K : d.N, d.ldb, k.ldb, es);
       B = wb;
+    }
+    if (d.a_type == FRISK_DT_I8) {   // both in one launch
+      if (int rc = launch_repack(ja, jb, pl->sm_count, st)) return rc;
+    } else {
+      for (const RepackJob* j : {&ja, &jb})
+        if (j->rows)
+          if (int rc = launch_repack(*j, RepackJob{}, pl->sm_count, st)) return rc;
     }
     workspace = w + repack_bytes;   // what follows is the kernels' own scratch
   }
