@@ -1301,6 +1301,15 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
       if (d.k_split == 3) {   // forced: four pairs per cluster where the SMs allow, else two
         for (int sp : {4, 2})
           if (!pcl && pair_ok && tiles128 * 2 * sp <= (uint64_t)pl->sm_count && kbs >= 8u * sp) pcl = sp;
+      } else if (d.k_split == 0 && pair_ok && d.a_type == FRISK_DT_I8 && kbs <= 128) {
+        // Integers, measured again (their k-blocks are twice as deep): C rows off the 16-byte grid leave
+        // this kernel element by element (700 x 300 x 8192, bf16 C: 21.2 us, single-CTA clusters 11.7),
+        // and from twelve tiles on up to 45 % of padding rows pay (333 x 1000 x 8192 17.8 -> 13.3 us,
+        // 300 x 1000 x 8192 17.8 -> 13.3; 129 x 1000 x 8192, half padding, 10.8 -> 12.2: left out).
+        const bool c_rows = (d.ldc * elem_size(d.c_type)) % 16 == 0;
+        const bool padded = 20 * (rows_pad - d.M) <= 9 * rows_pad && 4 * (cols_pad - d.N) <= cols_pad;
+        if (c_rows && full_tiles && tiles128 >= 6 && tiles128 <= 9 && kbs >= 32) pcl = 4;
+        else if (c_rows && padded && tiles128 >= 12 && tiles128 * 4 <= (uint64_t)pl->sm_count && kbs >= 48) pcl = 2;
       } else if (d.k_split == 0 && pair_ok && full_tiles && kbs <= 128) {
         if (tiles128 >= 6 && tiles128 <= 9 && kbs >= 32) pcl = 4;
         else if (tiles128 >= 12 && tiles128 * 4 <= (uint64_t)pl->sm_count && kbs >= 48) pcl = 2;
