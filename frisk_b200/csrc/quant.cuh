@@ -440,76 +440,216 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   }
 }
 
-// The same for rows at any alignment and width: the threads of a row take neighbouring ELEMENTS, the
-// e-th of a thread lying e x (threads per row) further on, so that every access of a warp is one run
-// of 32 elements.  Elements past the end of the row are zeros.
+// ---- the same for rows at any alignment and width -----------------------------------------------
+// Memory is still touched in aligned words of 16 bytes (8 for q): a group that starts inside a word is
+// shifted together from the words it lies in, and a stored word from the end of one lane's group and
+// the start of the next one's.
+
+// The words of v from byte `by` on (below 16): W of them, out of W + 4.
+template <int W>
+__device__ __forceinline__ void shift_words(uint32_t (&v)[W + 4], uint32_t by) {
+#pragma unroll
+  for (int i = 0; i < W + 2; ++i) v[i] = by & 8u ? v[i + 2] : v[i];
+#pragma unroll
+  for (int i = 0; i < W + 1; ++i) v[i] = by & 4u ? v[i + 1] : v[i];
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8u * (by & 3u));
+}
+
+// Elements c .. c + 7 of a row of a buffer that spans [lo, hi); zeros past the row's end.  A group that
+// crosses that end, or whose words reach out of the buffer, is read element by element.
+template <typename T>
+struct Ragged {
+  uint32_t w[2 * sizeof(T) + 4];
+  uint32_t by;   // where the group starts in w
+};
+template <typename T>
+__device__ __forceinline__ void load8_ragged(Ragged<T>& g, const T* row, int c, int cols, const void* lo, const void* hi) {
+  constexpr int W = 2 * sizeof(T);   // 32-bit words of a group
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+  g.by = (uint32_t)(at & 15u);
+  const uint4* p = reinterpret_cast<const uint4*>(at - g.by);
+  if (c + 8 <= cols && p >= lo && p + W / 4 + 1 <= hi) {
+#pragma unroll
+    for (int i = 0; i < W / 4 + 1; ++i) {
+      const uint4 v = p[i];
+      g.w[4 * i] = v.x;
+      g.w[4 * i + 1] = v.y;
+      g.w[4 * i + 2] = v.z;
+      g.w[4 * i + 3] = v.w;
+    }
+    return;
+  }
+  g.by = 0;
+  constexpr int kPer = 4 / (int)sizeof(T);   // elements of a word
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    uint32_t x = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (c + i * kPer + k < cols) {
+        const T e = row[c + i * kPer + k];
+        uint32_t bits;
+        if constexpr (sizeof(T) == 2) bits = *reinterpret_cast<const uint16_t*>(&e);
+        else bits = *reinterpret_cast<const uint32_t*>(&e);
+        x |= bits << (16 * k);
+      }
+    }
+    g.w[i] = x;
+  }
+}
+template <typename T>
+__device__ __forceinline__ Eight<T> take8(Ragged<T>& g) {
+  constexpr int W = 2 * sizeof(T);
+  shift_words<W>(g.w, g.by);
+  Eight<T> r;
+#pragma unroll
+  for (int i = 0; i < W / 4; ++i) r.w[i] = make_uint4(g.w[4 * i], g.w[4 * i + 1], g.w[4 * i + 2], g.w[4 * i + 3]);
+  return r;
+}
+
+// A warp's 32 x NV neighbouring groups into a row: lane L's i-th group, w[i] (elements of ES bytes), is
+// elements c0 + 8 (32 i + L) and on.  A lane stores the units (aligned words) that end in its group; the
+// first of them begins in the group to the left.  What no unit covers -- the first group's start, the
+// last one's end, the end of the row -- goes element by element, a group at a time.
+template <int ES, int NV>
+__device__ __forceinline__ void store_ragged(unsigned char* row, int c0, int cols, const uint32_t (&w)[NV][2 * ES], int lane) {
+  constexpr int W = 2 * ES;                 // words of a group
+  constexpr int U = W < 4 ? W : 4;          // words of a unit
+  constexpr int EU = 4 * U / ES;            // elements of a unit
+  const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(row) % (4 * U));   // groups are whole units long
+  const int o = (int)off / ES;              // elements of the left group in a group's first unit
+  uint32_t carry[U] = {};                   // lane 0: the end of lane 31's group before
+  uint32_t need[NV];                        // elements of the group that no unit covers
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + 8 * (32 * i + lane);
+    const int have = max(0, min(8, cols - c)), have_next = cols - (c + 8);
+    uint32_t v[W + 4] = {};
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const uint32_t left = __shfl_sync(0xffffffffu, w[i][W - U + k], (lane + 31) & 31);
+      v[k] = lane == 0 ? carry[k] : left;
+      carry[k] = left;
+    }
+#pragma unroll
+    for (int k = 0; k < W; ++k) v[U + k] = w[i][k];
+    if (off == 0) {
+#pragma unroll
+      for (int k = 0; k < W; ++k) v[k] = w[i][k];
+    } else {   // from byte 4 U - off on (1 .. 4 U - 1)
+      shift_words<W>(v, 4 * U - off);
+    }
+    unsigned char* first = row + (int64_t)c * ES - off;
+    uint32_t covered = 0;
+#pragma unroll
+    for (int u = 0; u < W / U; ++u) {
+      if ((u > 0 || lane > 0 || i > 0 || o == 0) && (u + 1) * EU - o <= have) {
+        if constexpr (U == 4) *reinterpret_cast<uint4*>(first + 16 * u) = make_uint4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+        else *reinterpret_cast<uint2*>(first) = make_uint2(v[0], v[1]);
+        covered |= (((1u << EU) - 1u) << (u * EU)) >> o;
+      }
+    }
+    // (the right group's first unit)
+    if (o > 0 && (lane < 31 || i < NV - 1) && have_next >= EU - o) covered |= 0xffu << (8 - o);
+    need[i] = ((1u << have) - 1u) & ~covered;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    uint32_t lanes = __ballot_sync(0xffffffffu, need[i] != 0);
+    while (lanes) {
+      const int src = __ffs(lanes) - 1;
+      lanes &= lanes - 1;
+      const uint32_t which = __shfl_sync(0xffffffffu, need[i], src);
+      uint32_t x = 0;   // the word of the group with element `lane`
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const uint32_t y = __shfl_sync(0xffffffffu, w[i][k], src);
+        if (lane * ES / 4 == k) x = y;
+      }
+      if (lane < 8 && (which >> lane & 1u)) {
+        unsigned char* dst = row + (int64_t)(c0 + 8 * (32 * i + src) + lane) * ES;
+        x >>= 8 * (lane * ES & 3);
+        if constexpr (ES == 1) *dst = (uint8_t)x;
+        else if constexpr (ES == 2) *reinterpret_cast<uint16_t*>(dst) = (uint16_t)x;
+        else *reinterpret_cast<uint32_t*>(dst) = x;
+      }
+    }
+  }
+}
+
 template <typename TIn, typename TW, int KIND, int NV>
 __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params p) {
   __shared__ float s_sum[32];
   __shared__ uint32_t s_max[32];
-  constexpr int NE = 8 * NV;
-  const int t = threadIdx.x, step = blockDim.x, lane = t & 31, wpr = step >> 5;
-  const int slot = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp = slot * wpr + (t >> 5);
+  const int t = threadIdx.x, lane = t & 31, wpr = blockDim.x >> 5;
+  const int slot = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp_in_row = __shfl_sync(0xffffffffu, t >> 5, 0);
   const int64_t r = (int64_t)blockIdx.x * blockDim.y + slot;
-  const int left = r < p.rows ? (int)p.cols - t : 0;   // element e exists where e * step < left
-  const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
-  const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
+  const bool live = r < p.rows;
+  const int cols = live ? (int)p.cols : 0, c0 = warp_in_row * 256 * NV;   // the warp's first element
+  const TIn* x0 = static_cast<const TIn*>(p.x);
+  const TIn* o0 = static_cast<const TIn*>(p.other);
   const TW* w = static_cast<const TW*>(p.weight);
-  TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
-  uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
-  auto at = [&](int e) { return (uint32_t)(t + e * step); };
+  const TIn* x = x0 + r * p.ldx;
+  const TIn* o = o0 ? o0 + r * p.ldo : nullptr;
 
-  TIn rx[NE], ro[NE];
+  Ragged<TIn> rx[NV], ro[NV];
 #pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    rx[e] = ro[e] = from_float<TIn>(0.f);
-    if (e * step < left) rx[e] = x[at(e)];
-  }
-  if (KIND != FRISK_QUANT_PLAIN && o) {
-#pragma unroll
-    for (int e = 0; e < NE; ++e)
-      if (e * step < left) ro[e] = o[at(e)];
+  for (int i = 0; i < NV; ++i) {
+    const int c = c0 + 8 * (32 * i + lane);
+    load8_ragged(rx[i], x, c, cols, x0, x0 + (p.rows - 1) * p.ldx + p.cols);
+    if (KIND != FRISK_QUANT_PLAIN && o) load8_ragged(ro[i], o, c, cols, o0, o0 + (p.rows - 1) * p.ldo + p.cols);
   }
   f2 g[NV][4];
   f2 sums = 0;
   float top = 0.f;
+  uint32_t hw[NV][2 * sizeof(TIn)];   // h as stored
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    Eight<TIn> ex = take8(rx[i]), eo = ex;
+    if (KIND != FRISK_QUANT_PLAIN && o) eo = take8(ro[i]);
+    group_values<TIn, KIND>(
+        ex, eo, o != nullptr,
+        [&](f2 (&v)[4]) {
+          if (w) {
+            Ragged<TW> rw;
+            load8_ragged(rw, w, c0 + 8 * (32 * i + lane), cols, w, w + p.cols);
+            unpack8(take8(rw), v);
+          }
+          return w != nullptr;
+        },
+        [&](const f2 (&h)[4]) {
+          Eight<TIn> e;
+          store8(reinterpret_cast<TIn*>(e.w), h);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int e = 8 * i + 2 * j;
-      f2 v = pack2(to_float<TIn>(rx[e]), to_float<TIn>(rx[e + 1]));
-      const f2 u = pack2(to_float<TIn>(ro[e]), to_float<TIn>(ro[e + 1]));
-      if (KIND == FRISK_QUANT_SILU_MUL) v = silu_mul2(v, u);
-      if (KIND == FRISK_QUANT_RMSNORM) {
-        v = add2(v, u);   // (x and the residual have been read: h may go to either)
-        sums = fma2(v, v, sums);
-        if (so) {
-          if (e * step < left) so[at(e)] = from_float<TIn>(lo2(v));
-          if ((e + 1) * step < left) so[at(e + 1)] = from_float<TIn>(hi2(v));
-        }
-        if (w) {
-          TW w0 = from_float<TW>(0.f), w1 = w0;
-          if (e * step < left) w0 = w[at(e)];
-          if ((e + 1) * step < left) w1 = w[at(e + 1)];
-          v = mul2(v, pack2(to_float<TW>(w0), to_float<TW>(w1)));
-        }
-      }
-      top = abs_max(v, top);
-      g[i][j] = v;
-    }
+          for (int k = 0; k < (int)sizeof(TIn) / 2; ++k) {
+            hw[i][4 * k] = e.w[k].x;
+            hw[i][4 * k + 1] = e.w[k].y;
+            hw[i][4 * k + 2] = e.w[k].z;
+            hw[i][4 * k + 3] = e.w[k].w;
+          }
+        },
+        g[i], sums, top);
+  }
+  if (KIND == FRISK_QUANT_RMSNORM && p.sum_out) {
+    // h may take the place of x or of the residual, and what this warp stores lies in words that the
+    // row's other warps read: they have to have read them
+    __syncthreads();
+    store_ragged<sizeof(TIn), NV>(reinterpret_cast<unsigned char*>(static_cast<TIn*>(p.sum_out) + r * p.lds), c0, cols, hw, lane);
+  }
   float sum = lo2(sums) + hi2(sums);
   uint32_t mx = __float_as_uint(top);
-  row_fold<KIND>(sum, mx, s_sum, s_max, warp, lane, slot, wpr);
-  if (r >= p.rows) return;
+  row_fold<KIND>(sum, mx, s_sum, s_max, slot * wpr + warp_in_row, lane, slot, wpr);
+  if (!live) return;
   divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  uint32_t qw[NV][2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const uint2 b = encode8x8(g[i], p.q_type);
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if ((8 * i + k) * step < left) q[at(8 * i + k)] = (uint8_t)((k < 4 ? b.x : b.y) >> (8 * (k & 3)));
+    qw[i][0] = b.x;
+    qw[i][1] = b.y;
   }
+  store_ragged<1, NV>(static_cast<unsigned char*>(p.q) + r * p.ldq, c0, cols, qw, lane);
 }
 
 // ---- many gated rows: streamed through shared memory ---------------------------------------------
