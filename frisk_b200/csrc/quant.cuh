@@ -472,11 +472,10 @@ __device__ __forceinline__ void load8_ragged(Ragged<T>& g, const T* row, int c, 
   if (c + 8 <= cols && p >= lo && p + W / 4 + 1 <= hi) {
 #pragma unroll
     for (int i = 0; i < W / 4 + 1; ++i) {
-      const uint4 v = p[i];
-      g.w[4 * i] = v.x;
-      g.w[4 * i + 1] = v.y;
-      g.w[4 * i + 2] = v.z;
-      g.w[4 * i + 3] = v.w;
+      asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(g.w[4 * i]), "=r"(g.w[4 * i + 1]), "=r"(g.w[4 * i + 2]), "=r"(g.w[4 * i + 3])
+                   : "l"(p + i)
+                   : "memory");
     }
     return;
   }
@@ -592,6 +591,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
   const TW* w = static_cast<const TW*>(p.weight);
   const TIn* x = x0 + r * p.ldx;
   const TIn* o = o0 ? o0 + r * p.ldo : nullptr;
+  const bool w_aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 
   Ragged<TIn> rx[NV], ro[NV];
 #pragma unroll
@@ -611,9 +611,12 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
     group_values<TIn, KIND>(
         ex, eo, o != nullptr,
         [&](f2 (&v)[4]) {
-          if (w) {
+          const int c = c0 + 8 * (32 * i + lane);
+          if (w && w_aligned && c + 8 <= cols) {
+            unpack8(load8_shared_by_rows(w + c), v);
+          } else if (w) {
             Ragged<TW> rw;
-            load8_ragged(rw, w, c0 + 8 * (32 * i + lane), cols, w, w + p.cols);
+            load8_ragged(rw, w, c, cols, w, w + p.cols);
             unpack8(take8(rw), v);
           }
           return w != nullptr;
