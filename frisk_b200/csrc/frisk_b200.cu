@@ -13,6 +13,7 @@
 #include <string>
 
 #include "abi_internal.h"
+#include "gemm_i8_rows.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_tcgen05.cuh"
 #include "gemm_tcgen05_pair.cuh"
@@ -1046,6 +1047,84 @@ int launch_simt(const frisk_gemm_desc& d, const void* A, const void* B, void* C,
   }
 }
 
+// The integer gemm of a few tokens (gemm_i8_rows.cuh): K innermost in both operands, 16-byte rows.
+bool i8_rows_ok(const frisk_gemm_desc& d) {
+  return d.a_type == FRISK_DT_I8 && d.M <= frisk::kI8RowsMaxM && tcgen05_eligible(d) && !d.row_reduce;
+}
+
+// Tiles of 16 weight rows per CTA, and chunks in flight per warp.  One tile and four chunks keep the
+// most bytes in flight per row and suit grids that the device holds at once (two CTAs per SM); larger
+// grids take fewer chunks for more CTAs beside one another, and two tiles, which halve the tokens'
+// traffic, where K is long enough to hide the longer fold.  Measured, one token, N x K: 4096 x 4096 as
+// (1, 4) / (1, 3) / (2, 2) 3.5 / 4.4 / 5.1 us, 28672 x 4096 21.8 / 20.7 / 21.6, 8192 x 8192 13.8 / 14.0 /
+// 12.9, 1000 x 4096 3.1 / 2.9 / 3.7; 16 tokens: 4096 x 4096 as (1, 4) / (2, 2) / (2, 3) 6.1 / 6.6 / 4.6,
+// 8192 x 8192 20.6 / 15.4 / 17.4, 1024 x 8192 4.8 / 7.0 / 7.3.
+void i8_rows_shape(const frisk_gemm_desc& d, int sms, int* tiles, int* stages) {
+  if (d.M <= 8) {
+    const bool wide = d.N >= 32ll * sms && d.K >= 8192;
+    *tiles = wide ? 2 : 1;
+    *stages = wide ? 2 : d.N <= 32ll * sms ? 4 : 3;
+  } else {
+    *tiles = d.N < 16ll * sms ? 1 : 2;
+    *stages = *tiles == 1 ? 4 : d.N <= 32ll * sms ? 3 : 2;
+  }
+}
+
+template <typename TC, int R, int MT, int S> struct I8RowsKernelTag {};
+template <typename TC, int R, int MT, int S>
+int launch_i8_rows_trs(const frisk::I8RowsParams& p, int device, cudaStream_t st) {
+  auto kern = frisk::gemm_i8_rows_kernel<TC, R, MT, S>;
+  if (int rc = ensure_dyn_smem<I8RowsKernelTag<TC, R, MT, S>>(kern, device)) return rc;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.N + 16 * R - 1) / (16 * R)), 1, 1);
+  cfg.blockDim = dim3(32 * frisk::kI8RowsWarps, 1, 1);
+  cfg.dynamicSmemBytes = frisk::i8_rows_smem<R, MT, S>();
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FRISK_CUDA(cudaLaunchKernelEx(&cfg, kern, p));
+  return FRISK_OK;
+}
+template <typename TC>
+int launch_i8_rows_t(const frisk::I8RowsParams& p, int tiles, int stages, int device, cudaStream_t st) {
+  switch (100 * (p.M <= 8 ? 1 : 2) + 10 * tiles + stages) {   // the shapes i8_rows_shape picks
+    case 113: return launch_i8_rows_trs<TC, 1, 1, 3>(p, device, st);
+    case 114: return launch_i8_rows_trs<TC, 1, 1, 4>(p, device, st);
+    case 122: return launch_i8_rows_trs<TC, 2, 1, 2>(p, device, st);
+    case 214: return launch_i8_rows_trs<TC, 1, 2, 4>(p, device, st);
+    case 222: return launch_i8_rows_trs<TC, 2, 2, 2>(p, device, st);
+    case 223: return launch_i8_rows_trs<TC, 2, 2, 3>(p, device, st);
+    default: return FRISK_ERR_UNSUPPORTED;
+  }
+}
+int launch_i8_rows(const frisk_gemm_plan* pl, const void* A, const void* B, void* C, const float* sa, const float* sb,
+                   cudaStream_t st) {
+  frisk::I8RowsParams p;
+  p.A = static_cast<const int8_t*>(A);
+  p.B = static_cast<const int8_t*>(B);
+  p.C = C;
+  p.scale_a = sa;
+  p.scale_b = sb;
+  p.lda = pl->kd.lda;
+  p.ldb = pl->kd.ldb;
+  p.ldc = pl->d.ldc;
+  p.M = (int32_t)pl->d.M;
+  p.N = (int32_t)pl->d.N;
+  p.K = (int32_t)pl->d.K;
+  p.clear_accum = pl->d.clear_accum;
+  const int tiles = pl->info.tile_n / 16;
+  switch (pl->d.c_type) {
+    case FRISK_DT_F32: return launch_i8_rows_t<float>(p, tiles, pl->info.stages, pl->device, st);
+    case FRISK_DT_F16: return launch_i8_rows_t<__half>(p, tiles, pl->info.stages, pl->device, st);
+    case FRISK_DT_BF16: return launch_i8_rows_t<__nv_bfloat16>(p, tiles, pl->info.stages, pl->device, st);
+    default: return FRISK_ERR_UNSUPPORTED;
+  }
+}
+
 size_t a_bytes(const frisk_gemm_desc& d) {
   return (size_t)(d.transA ? d.K : d.M) * d.lda * elem_size(d.a_type);
 }
@@ -1112,7 +1191,7 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
     return FRISK_ERR_INVALID_ARGUMENT;
   if (d.tile_n != 0 && d.tile_n != 64 && d.tile_n != 128 && d.tile_n != 256)
     return FRISK_ERR_INVALID_ARGUMENT;
-  if (d.force_kernel < 0 || d.force_kernel > 5 || d.stages < 0 || d.num_ctas < 0 || d.band_tiles < 0)
+  if (d.force_kernel < 0 || d.force_kernel > 6 || d.stages < 0 || d.num_ctas < 0 || d.band_tiles < 0)
     return FRISK_ERR_INVALID_ARGUMENT;
   if (d.epilogue < 0 || d.epilogue > 4 || d.row_reduce < 0 || d.row_reduce > 4 ||
       d.panel_tiles < 0 || d.l2_hints < 0 || d.l2_hints > 3 || d.k_split < -1 || d.k_split > 3)
@@ -1200,7 +1279,7 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
   if (d.force_kernel) {
     kind = d.force_kernel - 1;
     if ((kind == FRISK_KERNEL_TCGEN05 && !tc_ok) || (kind == FRISK_KERNEL_SKINNY && !skinny_ok) ||
-        (kind == FRISK_KERNEL_TCGEN05_PAIR && !pair_ok)) {
+        (kind == FRISK_KERNEL_TCGEN05_PAIR && !pair_ok) || (kind == FRISK_KERNEL_I8_ROWS && !i8_rows_ok(d))) {
       delete pl;
       return tc_ok ? FRISK_ERR_UNSUPPORTED : FRISK_ERR_MISALIGNED;
     }
@@ -1224,7 +1303,10 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
       if (const char* want_pair = getenv("FRISK_B200_PAIR")) use_pair = want_pair[0] == '1';
 #endif
     }
-    kind = (skinny_ok && !d.row_reduce) ? FRISK_KERNEL_SKINNY
+    // (16 tokens against 28672 of K: 43.4 us here, 40.7 in the few-row plan)
+    const bool i8_rows = i8_rows_ok(d) && !d.num_ctas && (d.M <= 8 || d.K <= 16384);
+    kind = i8_rows ? FRISK_KERNEL_I8_ROWS
+           : (skinny_ok && !d.row_reduce) ? FRISK_KERNEL_SKINNY
            : use_pair                    ? FRISK_KERNEL_TCGEN05_PAIR
            : tc_ok                       ? FRISK_KERNEL_TCGEN05
                                          : FRISK_KERNEL_SIMT;
@@ -1236,7 +1318,18 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
                    "inputs with 16-byte row pitches)";
     return FRISK_ERR_UNSUPPORTED;
   }
-  if (kind == FRISK_KERNEL_SIMT) {
+  if (kind == FRISK_KERNEL_I8_ROWS) {
+    frisk_gemm_plan_info& in = pl->info;
+    in.kernel = FRISK_KERNEL_I8_ROWS;
+    int tiles = 1, stages = 1;
+    i8_rows_shape(d, pl->sm_count, &tiles, &stages);
+    in.tile_m = frisk::kI8RowsMaxM;
+    in.tile_n = 16 * tiles;
+    in.tile_k = 128;
+    in.stages = stages;
+    in.num_ctas = (int)((d.N + in.tile_n - 1) / in.tile_n);
+    in.launches = 1;
+  } else if (kind == FRISK_KERNEL_SIMT) {
     pl->info.kernel = FRISK_KERNEL_SIMT;
     pl->info.cuda_core_reason = d.force_kernel ? FRISK_TC_FORCED : tcgen05_ineligible_reason(d);
     // the same choice launch_simt_in makes: 32-row tiles when 64-row tiles would not fill the SMs
@@ -1391,7 +1484,8 @@ int frisk_b200_gemm_plan_operand_layout(const frisk_gemm_plan* pl, int32_t opera
                                         frisk_tma_params* layout, uint64_t* umma_desc_base,
                                         int32_t* tma_boxes_per_stage) {
   if (!pl || operand < 0 || operand > 1) return FRISK_ERR_INVALID_ARGUMENT;
-  if (pl->info.kernel == FRISK_KERNEL_SIMT) return FRISK_ERR_UNSUPPORTED;  // nothing is staged by TMA
+  if (pl->info.kernel == FRISK_KERNEL_SIMT || pl->info.kernel == FRISK_KERNEL_I8_ROWS)
+    return FRISK_ERR_UNSUPPORTED;  // nothing is staged by TMA
   const frisk::OperandParams& o = operand ? pl->gp.b : pl->gp.a;
   if (layout) *layout = operand ? pl->lay_b : pl->lay_a;
   if (umma_desc_base) *umma_desc_base = o.desc_base;
@@ -1538,6 +1632,7 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
   }
   if (pl->info.kernel == FRISK_KERNEL_SIMT || !ptr_aligned)
     return launch_simt(d, A0, B0, C, sa, sb, st);  // the CUDA-core kernel has no alignment rule
+  if (pl->info.kernel == FRISK_KERNEL_I8_ROWS) return launch_i8_rows(pl, A, B, C, sa, sb, st);
 
   const bool swap = pl->info.kernel == FRISK_KERNEL_SKINNY;
   const size_t own_ws_bytes = pl->ws_bytes - repack_bytes;

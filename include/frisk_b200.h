@@ -73,9 +73,11 @@ typedef enum {
   FRISK_KERNEL_TCGEN05 = 1, /* TMA + tcgen05.mma, accumulators in TMEM, whole-tile output   */
   FRISK_KERNEL_SKINNY = 2,  /* few rows (M <= 128): operands swapped, K split over a cluster / SMs */
   FRISK_KERNEL_TCGEN05_PAIR = 3, /* CTA pairs with two-SM MMAs on 256 x tile_n output tiles  */
-  FRISK_KERNEL_TF32X3 = 4   /* fp32 inputs and C: A and B split into tf32 hi + lo parts in the
+  FRISK_KERNEL_TF32X3 = 4,  /* fp32 inputs and C: A and B split into tf32 hi + lo parts in the
                                workspace, three products in one tensor-core GEMM (fp32-level
                                accuracy: relative error about 1e-6); larger problems only      */
+  FRISK_KERNEL_I8_ROWS = 5  /* 8-bit integers, at most 16 tokens: the weights streamed once past
+                               warp-level MMAs                                                */
 } frisk_kernel_kind;
 
 /*

@@ -146,14 +146,27 @@ PLANS = [
     (512, 768, 640, "tcgen05_pair", {"epilogue": 4}),
     (128, 256, 256, "tcgen05", {"force_kernel": "tcgen05"}),
     (333, 200, 400, "tcgen05", {"force_kernel": "tcgen05", "tile_n": 64}),
-    (1, 4096, 4096, "skinny", {}),                                       # one token
-    (1, 256, 16, "skinny", {}),
-    (16, 8192, 1024, "skinny", {}),
+    (1, 4096, 4096, "i8_rows", {}),                                      # one token
+    (1, 256, 16, "i8_rows", {}),
+    (1, 1, 16, "i8_rows", {}),
+    (3, 37, 100, "i8_rows", {}),                                         # repacked, less than a chunk of K
+    (8, 100, 528, "i8_rows", {}),
+    (8, 4100, 528, "i8_rows", {}),
+    (5, 8192, 8192, "i8_rows", {}),                                      # two tiles of weight rows per CTA
+    (2, 300, 28672, "i8_rows", {}),
+    (9, 4100, 528, "i8_rows", {}),                                       # two tiles of tokens
+    (16, 8192, 1024, "i8_rows", {}),
+    (16, 512, 4096, "i8_rows", {}),
+    (13, 1000, 4099, "i8_rows", {}),
+    (16, 2048, 28672, "skinny", {}),
+    (1, 4096, 4096, "skinny", {"force_kernel": "skinny"}),
+    (1, 256, 16, "skinny", {"force_kernel": "skinny"}),
+    (16, 8192, 1024, "skinny", {"force_kernel": "skinny"}),
+    (16, 512, 4096, "skinny", {"force_kernel": "skinny"}),
     (33, 4100, 528, "skinny", {}),
     (64, 2048, 2048, "skinny", {}),
     (100, 8192, 512, "skinny", {}),
     (128, 8192, 1040, "skinny", {}),
-    (16, 512, 4096, "skinny", {}),
     (16, 8192, 1024, "skinny", {"num_ctas": 97}),                        # stream-K: partials in slots
     (24, 512, 8192, "skinny", {"num_ctas": 148}),                        # more partials of a tile than its list holds
     (512, 512, 4096, "tcgen05_pair", {"k_split": 3}),                    # K over the pairs of a cluster

@@ -60,11 +60,14 @@ def test_builder_and_parser_take_8_bit_integers():
 
 
 def test_kernel_families_and_the_fixed_scratch_entry_point():
-    for (M, N, K), kernel in (((8192, 8192, 8192), "tcgen05_pair"), ((16, 8192, 8192), "skinny"), ((1, 4096, 4096), "skinny"),
+    for (M, N, K), kernel in (((8192, 8192, 8192), "tcgen05_pair"), ((16, 8192, 8192), "i8_rows"), ((1, 4096, 4096), "i8_rows"),
+                              ((8, 8192, 8192), "i8_rows"), ((17, 8192, 8192), "skinny"),
                               ((128, 192, 256), "tcgen05")):
         p = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True)
         assert p.info["kernel_name"] == kernel and p.info["tile_k"] == 128, p.info
         p.close()
+    refused(-2, 17, 4096, 4096, W.I8, W.BF16, transB=True, force_kernel="i8_rows")      # at most 16 tokens
+    refused(-2, 8, 4096, 4096, W.BF16, W.BF16, transB=True, force_kernel="i8_rows")
     d = R.GemmDesc()     # its scratch adds fp32 partial sums: not for an exact product
     d.M, d.N, d.K, d.a_type, d.b_type, d.c_type, d.transB, d.clear_accum = 16, 512, 512, W.I8, W.I8, W.BF16, 1, 1
     assert R.lib().frisk_b200_gemm_skinny_static(d, 0x10000, 0x20000, 0x30000, None, None, None, None) == -2
