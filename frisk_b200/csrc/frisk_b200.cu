@@ -934,6 +934,71 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const RepackJob a, con
   }
 }
 
+// The transpose of an 8-bit operand stored with K outermost: src [k][mn] (any base and pitch) to dst
+// [mn][ld_dst], ld_dst a multiple of 128, zeros behind K.  A CTA turns a tile of 128 x 128 around in
+// shared memory, in blocks of 4 x 4 bytes: four words read along mn, eight byte permutations, four
+// words written along k (one block per thread and step, so both sides of memory see whole lines).
+__global__ void __launch_bounds__(256) transpose_bytes_kernel(const unsigned char* __restrict__ src,
+                                                              unsigned char* __restrict__ dst, int64_t k, int64_t mn,
+                                                              int64_t src_pitch, int64_t ld_dst, uint32_t tiles_k) {
+  __shared__ uint32_t tile[128][33];   // [mn][k / 4]
+  frisk::ptx::griddep_launch_dependents();
+  frisk::ptx::griddep_wait();
+  const int64_t m0 = (int64_t)(blockIdx.x / tiles_k) * 128, k0 = (int64_t)(blockIdx.x % tiles_k) * 128;
+  const bool words = ((reinterpret_cast<uintptr_t>(src) | (uintptr_t)src_pitch) & 3) == 0;
+  const int mb = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int kb = (threadIdx.x >> 5) + 8 * i;
+    const int64_t kk = k0 + 4 * kb, mm = m0 + 4 * mb;
+    uint32_t w[4] = {0, 0, 0, 0};   // rows kk .. kk + 3, columns mm .. mm + 3
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (kk + j >= k || mm >= mn) continue;
+      const unsigned char* p = src + (kk + j) * src_pitch + mm;
+      if (words && mm + 4 <= mn) {
+        w[j] = *reinterpret_cast<const uint32_t*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (mm + e < mn) w[j] |= (uint32_t)p[e] << (8 * e);
+      }
+    }
+    const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[0], w[1], 0x7362);
+    const uint32_t c = __byte_perm(w[2], w[3], 0x5140), d = __byte_perm(w[2], w[3], 0x7362);
+    tile[4 * mb][kb] = __byte_perm(a, c, 0x5410);
+    tile[4 * mb + 1][kb] = __byte_perm(a, c, 0x7632);
+    tile[4 * mb + 2][kb] = __byte_perm(b, d, 0x5410);
+    tile[4 * mb + 3][kb] = __byte_perm(b, d, 0x7632);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = (threadIdx.x >> 3) + 32 * i, c = (threadIdx.x & 7) * 4;
+    if (m0 + row < mn)
+      *reinterpret_cast<uint4*>(dst + (m0 + row) * ld_dst + k0 + 4 * c) =
+          make_uint4(tile[row][c], tile[row][c + 1], tile[row][c + 2], tile[row][c + 3]);
+  }
+}
+
+int launch_transpose_bytes(const void* src, void* dst, int64_t k, int64_t mn, int64_t ld_src, int64_t ld_dst, cudaStream_t st) {
+  const int64_t tiles_k = ld_dst / 128, tiles = tiles_k * ((mn + 127) / 128);
+  if (tiles > 0x7fffffff) return FRISK_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof cfg);
+  cfg.gridDim = dim3((unsigned)tiles, 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FRISK_CUDA(cudaLaunchKernelEx(&cfg, transpose_bytes_kernel, static_cast<const unsigned char*>(src),
+                                static_cast<unsigned char*>(dst), k, mn, ld_src, ld_dst, (uint32_t)tiles_k));
+  return FRISK_OK;
+}
+
 RepackJob repack_job(const void* src, void* dst, int64_t rows, int64_t cols, int64_t ld_src, int64_t ld_dst, int es) {
   RepackJob j;
   j.src = static_cast<const unsigned char*>(src);
@@ -1257,10 +1322,27 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
   // buffers, not the tensor cores: the plan copies such an operand into the workspace at a padded
   // pitch before every run (one more launch each; the copy reads and writes the operand once,
   // against a CUDA-core kernel about 100 x slower on the whole problem).
-  if (tcgen05_ineligible_reason(d) == FRISK_TC_PITCH && d.force_kernel != 1 + FRISK_KERNEL_SIMT) {
-    // (integers to whole 128-byte lines: rows that start off them cost the tile loads a third of their
-    // rate -- 333 x 1000 x 4112 at a pitch of 4112 bytes 15.6 us, at 4224 11.6 us)
-    const int64_t es = elem_size(d.a_type), q = (d.a_type == FRISK_DT_I8 ? 128 : 16) / es;
+  const int why_not = tcgen05_ineligible_reason(d);
+  if (d.a_type == FRISK_DT_I8 && (why_not == FRISK_TC_PITCH || why_not == FRISK_TC_FP8_ORDER) &&
+      d.force_kernel != 1 + FRISK_KERNEL_SIMT) {
+    // Integers: an operand stored with K outermost is transposed on the way, and pitches go to whole
+    // 128-byte lines (rows that start off them cost the tile loads a third of their rate -- 333 x 1000 x
+    // 4112 at a pitch of 4112 bytes 15.6 us, at 4224 11.6 us).
+    frisk_gemm_desc& k = pl->kd;
+    const int64_t kp = (d.K + 127) / 128 * 128;
+    if (d.transA || d.lda % 16) {
+      k.transA = 0;
+      k.lda = kp;
+      pl->repack_a_bytes = ((size_t)d.M * kp + 255) / 256 * 256;
+    }
+    if (!d.transB || d.ldb % 16) {
+      k.transB = 1;
+      k.ldb = kp;
+      pl->repack_b_bytes = ((size_t)d.N * kp + 255) / 256 * 256;
+    }
+    d = k;
+  } else if (why_not == FRISK_TC_PITCH && d.force_kernel != 1 + FRISK_KERNEL_SIMT) {
+    const int64_t es = elem_size(d.a_type), q = 16 / es;
     frisk_gemm_desc& k = pl->kd;
     if ((d.lda * es) % 16) {
       k.lda = ((d.transA ? d.M : d.K) + q - 1) / q * q;
@@ -1474,8 +1556,10 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
     pl->kd = pl->d;
   }
   pl->ws_bytes += pl->repack_a_bytes + pl->repack_b_bytes;
+  // (integer operands that are only copied share a launch)
   const int repacked = (pl->repack_a_bytes ? 1 : 0) + (pl->repack_b_bytes ? 1 : 0);
-  pl->info.launches += pl->d.a_type == FRISK_DT_I8 ? std::min(repacked, 1) : repacked;
+  const bool one_launch = pl->d.a_type == FRISK_DT_I8 && !pl->d.transA && pl->d.transB;
+  pl->info.launches += one_launch ? std::min(repacked, 1) : repacked;
   *out = pl;
   return FRISK_OK;
 }
@@ -1598,18 +1682,27 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
     if ((uintptr_t)workspace % 16) return FRISK_ERR_MISALIGNED;
     const int es = elem_size(d.a_type);
     char* w = static_cast<char*>(workspace);
-    RepackJob ja{}, jb{};
+    RepackJob ja{}, jb{};   // copies; transposes go at once
     if (pl->repack_a_bytes) {
-      ja = repack_job(A, w, d.transA ? d.K : d.M, d.transA ? d.M : d.K, d.lda, k.lda, es);
+      if (d.transA && !k.transA) {
+        if (int rc = launch_transpose_bytes(A, w, d.K, d.M, d.lda, k.lda, st)) return rc;
+      } else {
+        ja = repack_job(A, w, d.transA ? d.K : d.M, d.transA ? d.M : d.K, d.lda, k.lda, es);
+      }
       A = w;
     }
     if (pl->repack_b_bytes) {
       char* wb = w + pl->repack_a_bytes;
-      jb = repack_job(B, wb, d.transB ? d.N : d.K, d.transB ? d.K : d.N, d.ldb, k.ldb, es);
+      if (!d.transB && k.transB) {
+        if (int rc = launch_transpose_bytes(B, wb, d.K, d.N, d.ldb, k.ldb, st)) return rc;
+      } else {
+        jb = repack_job(B, wb, d.transB ? d.N : d.K, d.transB ? d.K : d.N, d.ldb, k.ldb, es);
+      }
       B = wb;
     }
     if (d.a_type == FRISK_DT_I8) {   // both in one launch
-      if (int rc = launch_repack(ja, jb, pl->sm_count, st)) return rc;
+      if (ja.rows || jb.rows)
+        if (int rc = launch_repack(ja, jb, pl->sm_count, st)) return rc;
     } else {
       for (const RepackJob* j : {&ja, &jb})
         if (j->rows)
@@ -1642,8 +1735,8 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
   }
   frisk::GemmParams g = pl->gp;
   if (A != pl->cached_a || B != pl->cached_b) {
-    OperandView va{A, d.M, d.K, k.lda, d.transA != 0};
-    OperandView vb{B, d.N, d.K, k.ldb, d.transB == 0};
+    OperandView va{A, d.M, d.K, k.lda, k.transA != 0};
+    OperandView vb{B, d.N, d.K, k.ldb, k.transB == 0};
     const OperandView& ra = swap ? vb : va;  // a-role: the 128-row operand
     const OperandView& rb = swap ? va : vb;
     int rc = encode_operand_map(&pl->tmap_a, ra, d.a_type, g.a.box_mn, g.bk_elems, pl->lay_a.swizzle_bytes);

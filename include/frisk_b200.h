@@ -160,7 +160,8 @@ enum {
   FRISK_TC_INPUT_TYPE = 1, /* A and B are not fp16, bf16 or e4m3                              */
   FRISK_TC_PITCH = 2,      /* a row pitch of A or B is not a multiple of 16 bytes (TMA rule)   */
   FRISK_TC_EXTENT = 3,     /* M, N or K is 2^31 or more                                        */
-  FRISK_TC_FP8_ORDER = 4,  /* e4m3 operands are taken K-inner only (transA = 0, transB = 1)    */
+  FRISK_TC_FP8_ORDER = 4,  /* e4m3 operands are taken K-inner only (transA = 0, transB = 1); integers
+                              in another order are transposed into the workspace before every run */
   FRISK_TC_FORCED = 5      /* desc.force_kernel asked for the CUDA-core kernel                 */
 };
 
@@ -175,8 +176,9 @@ int frisk_b200_gemm_plan_info(const frisk_gemm_plan* plan, frisk_gemm_plan_info*
  * plans (shapes whose tiles cannot be covered by thread-block clusters), plans with a fused row
  * reduce (one fp32 per row and half tile), K-planes plans (one fp32 copy of C per K part, at
  * most 20 MB), 3xTF32 plans (twice the bytes of A and B; 256-byte
- * aligned) and plans for an A or B whose row pitch is not a multiple of 16 bytes (a copy of that
- * operand at a padded pitch, made by one more launch before every run); `run` takes a NULL
+ * aligned), plans for an A or B whose row pitch is not a multiple of 16 bytes (a copy of that
+ * operand at a padded pitch, made by one more launch before every run) and integer plans for an A or B
+ * stored with K outermost (its transpose, made the same way); `run` takes a NULL
  * workspace when it is 0. */
 int frisk_b200_gemm_workspace_bytes(const frisk_gemm_plan* plan, size_t* out);
 

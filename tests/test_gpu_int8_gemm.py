@@ -267,3 +267,39 @@ def test_the_tensor_pipes_rate_can_be_measured():
     got = R.measure_mma_peak(W.I8, pair=True, k_blocks=1024, reps=5)
     assert got["tflops"] > 1000.0, got
     print(got)
+
+
+@pytest.mark.parametrize("M,N,K", [(200, 300, 1000), (16, 4096, 520), (1, 300, 130), (513, 257, 129)])
+def test_orders_through_the_workspace_and_the_cuda_core_kernel_agree(M, N, K):
+    """The transposed and copied operands' plans against the kernel that takes any order, bit for bit."""
+    for ta, tb, pad in ((False, False, (0, 0)), (True, True, (0, 0)), (True, False, (1, 3)), (False, True, (5, 0))):
+        a, b, _, _ = make(M, N, K, 13, full=True)
+        A, lda = stored(a, ta, pad[0])
+        B, ldb = stored(b, tb, pad[1])
+        out = []
+        for kw in ({}, {"force_kernel": "simt"}):
+            c = np.zeros((M, N), np.float32)
+            plan = R.GemmPlan(M, N, K, W.I8, W.F32, transA=ta, transB=tb, lda=lda, ldb=ldb, **kw)
+            plan.run_host(A, B, c)
+            plan.close()
+            out.append(c)
+        assert np.array_equal(out[0], out[1])
+        assert np.array_equal(out[0], (a.astype(np.int64) @ b.astype(np.int64)).astype(np.float32))
+
+
+def test_misaligned_bases_still_give_the_right_answer():
+    import torch
+    dev = torch.device("cuda:0")
+    M, N, K = 40, 300, 256
+    a, b, sa, sb = make(M, N, K, 14)
+    A, B = torch.zeros(M * K + 16, dtype=torch.int8, device=dev), torch.zeros(N * K + 16, dtype=torch.int8, device=dev)
+    A[3:3 + M * K] = torch.from_numpy(a.reshape(-1)).to(dev)
+    B[5:5 + N * K] = torch.from_numpy(np.ascontiguousarray(b.T).reshape(-1)).to(dev)
+    c = torch.zeros((M, N), dtype=torch.float32, device=dev)
+    plan = R.GemmPlan(M, N, K, W.I8, W.F32, transB=True, scales=True)
+    plan.run(A.data_ptr() + 3, B.data_ptr() + 5, c, torch.from_numpy(sa).to(dev), torch.from_numpy(sb).to(dev),
+             stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert plan.refresh_info()["cuda_core_runs"] == 1
+    plan.close()
+    check(c.cpu().numpy(), *expect(a, b, sa, sb), W.F32)

@@ -71,3 +71,19 @@ def test_kernel_families_and_the_fixed_scratch_entry_point():
     d = R.GemmDesc()     # its scratch adds fp32 partial sums: not for an exact product
     d.M, d.N, d.K, d.a_type, d.b_type, d.c_type, d.transB, d.clear_accum = 16, 512, 512, W.I8, W.I8, W.BF16, 1, 1
     assert R.lib().frisk_b200_gemm_skinny_static(d, 0x10000, 0x20000, 0x30000, None, None, None, None) == -2
+
+
+def test_other_orders_and_odd_pitches_are_brought_into_the_tensor_cores_order():
+    base = R.GemmPlan(512, 520, 256, W.I8, W.BF16, transB=True)
+    assert base.info["kernel_name"] == "tcgen05_pair" and base.workspace_bytes == 0 and base.info["launches"] == 1
+    base.close()
+    for kw, launches, ws in ((dict(transB=False), 2, 520 * 256), (dict(transA=True, transB=False), 3, (512 + 520) * 256),
+                             (dict(transA=True, transB=True), 2, 512 * 256),
+                             (dict(transB=True, lda=257, ldb=259), 2, (512 + 520) * 256),      # both copied by one launch
+                             (dict(transB=True, ldb=259), 2, 520 * 256)):
+        p = R.GemmPlan(512, 520, 256, W.I8, W.BF16, **kw)
+        assert p.info["kernel_name"] == "tcgen05_pair" and p.info["launches"] == launches and p.workspace_bytes == ws, (kw, p.info)
+        p.close()
+    p = R.GemmPlan(512, 520, 250, W.I8, W.BF16, transB=False, force_kernel="simt")
+    assert p.info["kernel_name"] == "simt" and p.workspace_bytes == 0 and p.info["launches"] == 1
+    p.close()
