@@ -69,6 +69,20 @@ cudaError_t allow_ring(int device) {
   return e;
 }
 
+cudaError_t go(void (*kern)(const Params), int64_t ctas, dim3 threads, size_t smem, const Params& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 template <typename TIn, typename TW, int KIND>
 cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   const int es = sizeof(TIn);
@@ -76,8 +90,7 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
                        rows_on(p.sum_out, p.lds, es, 16) && rows_on(p.q, p.ldq, 1, 8) && rows_on(p.weight, 0, 1, 16);
   constexpr int64_t kMaxCtas = 0x7fffffff;
   if (p.cols > 8 * 1024 * kMaxGroups || p.rows > kMaxCtas) {   // more than registers hold, or than a grid
-    frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND><<<(unsigned)std::min(p.rows, kMaxCtas), 256, 0, st>>>(p);
-    return cudaGetLastError();
+    return go(frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND>, std::min(p.rows, kMaxCtas), dim3(256), 0, p, st);
   }
   const int64_t groups = ceil_div(p.cols, 8);
   if constexpr (KIND == FRISK_QUANT_SILU_MUL) {
@@ -95,8 +108,7 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
       auto kern = full ? frisk_quant::quant_gated_stream_kernel<TIn, kMaxGroups, true>
                        : frisk_quant::quant_gated_stream_kernel<TIn, kMaxGroups, false>;
       if (const cudaError_t e = full ? allow_ring<TIn, true>(device) : allow_ring<TIn, false>(device)) return e;
-      kern<<<(unsigned)sms, dim3(32 * wpr, teams), stages * row, st>>>(p);
-      return cudaGetLastError();
+      return go(kern, sms, dim3(32 * wpr, teams), stages * row, p, st);
     }
   }
   // Many rows: four groups a thread, the most loads in flight per warp that registers allow (off the
@@ -111,22 +123,21 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   const int64_t ctas = ceil_div(p.rows, rows_per_cta);
   const dim3 threads(32 * wpr, rows_per_cta);
   const bool full = p.cols == 256ll * nv * wpr && p.rows % rows_per_cta == 0;
-  auto go = [&](auto kern) { kern<<<(unsigned)ctas, threads, 0, st>>>(p); };
   using namespace frisk_quant;
-  if (!aligned) {
-    switch (nv) {
-      case 1: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 1>); break;
-      case 2: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 2>); break;
-      default: go(quant_rows_unaligned_kernel<TIn, TW, KIND, 4>); break;
-    }
-    return cudaGetLastError();
-  }
-  switch (nv) {
-    case 1: full ? go(quant_rows_kernel<TIn, TW, KIND, 1, true>) : go(quant_rows_kernel<TIn, TW, KIND, 1, false>); break;
-    case 2: full ? go(quant_rows_kernel<TIn, TW, KIND, 2, true>) : go(quant_rows_kernel<TIn, TW, KIND, 2, false>); break;
-    default: full ? go(quant_rows_kernel<TIn, TW, KIND, 4, true>) : go(quant_rows_kernel<TIn, TW, KIND, 4, false>); break;
-  }
-  return cudaGetLastError();
+  void (*kern)(const Params);
+  if (!aligned)
+    kern = nv == 1   ? quant_rows_unaligned_kernel<TIn, TW, KIND, 1>
+           : nv == 2 ? quant_rows_unaligned_kernel<TIn, TW, KIND, 2>
+                     : quant_rows_unaligned_kernel<TIn, TW, KIND, 4>;
+  else if (full)
+    kern = nv == 1   ? quant_rows_kernel<TIn, TW, KIND, 1, true>
+           : nv == 2 ? quant_rows_kernel<TIn, TW, KIND, 2, true>
+                     : quant_rows_kernel<TIn, TW, KIND, 4, true>;
+  else
+    kern = nv == 1   ? quant_rows_kernel<TIn, TW, KIND, 1, false>
+           : nv == 2 ? quant_rows_kernel<TIn, TW, KIND, 2, false>
+                     : quant_rows_kernel<TIn, TW, KIND, 4, false>;
+  return go(kern, ctas, threads, 0, p, st);
 }
 
 template <typename TIn>

@@ -108,6 +108,14 @@ __device__ __forceinline__ float row_divisor(float sum_sq, uint32_t max_bits, in
   return tiny ? fmaxf(__fdiv_rn(kTinyScale, rstd), __uint_as_float(1u)) : d;
 }
 
+// Every kernel here is a programmatic dependent launch: it may be scheduled while the kernel before it
+// in the stream drains, waits here until that one's writes are visible, and lets the next one do the
+// same.
+__device__ __forceinline__ void after_the_kernel_before() {
+  frisk::ptx::griddep_launch_dependents();
+  frisk::ptx::griddep_wait();
+}
+
 // The plain form of the three kinds: a CTA per row, two passes over it, element by element.  Serves
 // any type, pitch, alignment and width.
 template <typename TIn, typename TW, int KIND>
@@ -115,6 +123,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
   __shared__ float s_sum[8];
   __shared__ uint32_t s_max[8];
   const TW* w = static_cast<const TW*>(p.weight);
+  after_the_kernel_before();
   for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
     const TIn* o = static_cast<const TIn*>(p.other);
@@ -400,6 +409,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   const TW* w = static_cast<const TW*>(p.weight);
   TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
 
+  after_the_kernel_before();
   Eight<TIn> rx[NV], ro[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -593,6 +603,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
   const TIn* o = o0 ? o0 + r * p.ldo : nullptr;
   const bool w_aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 
+  after_the_kernel_before();
   Ragged<TIn> rx[NV], ro[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -745,6 +756,9 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
       tags[s] = 0xffffffffu;   // (n is below that: checked when launching)
     }
     frisk::ptx::fence_mbar_init();
+  }
+  after_the_kernel_before();
+  if (threadIdx.x == 0 && threadIdx.y == 0) {
     for (int s = 0; s < stages && s < n; ++s) fetch(s, s);
   }
   __syncthreads();
