@@ -1114,7 +1114,7 @@ int launch_simt(const frisk_gemm_desc& d, const void* A, const void* B, void* C,
 
 // The integer gemm of a few tokens (gemm_i8_rows.cuh): K innermost in both operands, 16-byte rows.
 bool i8_rows_ok(const frisk_gemm_desc& d) {
-  return d.a_type == FRISK_DT_I8 && d.M <= frisk::kI8RowsMaxM && tcgen05_eligible(d) && !d.row_reduce;
+  return d.a_type == FRISK_DT_I8 && d.M <= frisk::kI8RowsMaxM && d.N < (1ll << 30) && tcgen05_eligible(d) && !d.row_reduce;
 }
 
 // Tiles of 16 weight rows per CTA, and chunks in flight per warp.  One tile and four chunks keep the

@@ -36,10 +36,11 @@ int check_desc(const frisk_quant_desc& d) {
       return fail(FRISK_ERR_UNSUPPORTED, "quant: the weight's type must be the input's or f32");
     if (!(d.eps >= 0.f) || std::isinf(d.eps)) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: eps must be finite and not negative");
   }
-  // rows and pitches below 2^40 keep every product of the two, in bytes, inside 64 bits
-  const int64_t lim = 1ll << 40;
-  if (d.rows >= lim || d.cols >= (1ll << 31) || d.ldx >= lim || d.ldo >= lim || d.lds >= lim || d.ldq >= lim)
-    return fail(FRISK_ERR_TOO_LARGE, "quant: 2^31 columns or more, or rows or pitches of 2^40 or more");
+  if (d.cols >= (1ll << 31)) return fail(FRISK_ERR_TOO_LARGE, "quant: 2^31 columns or more");
+  // every offset in bytes has to fit 63 bits (the widest packed pitch is 2 * cols of four bytes)
+  for (int64_t ld : {d.ldx, d.ldo, d.lds, d.ldq, 2 * d.cols})
+    if (ld > 0 && (unsigned __int128)d.rows * (unsigned __int128)ld >= ((unsigned __int128)1 << 60))
+      return fail(FRISK_ERR_TOO_LARGE, "quant: rows times a pitch is 2^60 or more");
   // (silu_mul with gate and up in one buffer needs 2 * cols; checked when the pointers are known)
   if ((d.ldx && d.ldx < d.cols) || (d.ldo && d.ldo < d.cols) || (d.lds && d.lds < d.cols) || (d.ldq && d.ldq < d.cols))
     return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: a pitch is shorter than a row");
@@ -189,6 +190,10 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
   // the sum may replace x or the residual, element for element
   if ((p.sum_out == p.x && p.sum_out && p.lds != p.ldx) || (p.sum_out == p.other && p.sum_out && p.lds != p.ldo))
     return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: sum_out in place of x or the residual needs the same pitch");
+  // q and scale lie by themselves (the caller answers for partial overlaps)
+  for (const void* b : {p.x, p.other, p.weight, (const void*)p.sum_out})
+    if (b == p.q || b == p.scale || p.q == p.scale)
+      return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: q and scale must not be one of the other buffers");
   int prev = -1;
   cudaError_t e;
   if (d.device >= 0) {

@@ -40,9 +40,10 @@ def test_descriptions_that_are_refused():
     for ld in ("ldx", "ldo", "lds", "ldq"):
         refused(INVALID, d(4, 8, W.BF16, W.I8, "rmsnorm", **{ld: 7}))
         refused(INVALID, d(4, 8, W.BF16, W.I8, "rmsnorm", **{ld: -8}))
-        refused(TOO_LARGE, d(4, 8, W.BF16, W.I8, "rmsnorm", **{ld: 1 << 40}))
+        refused(TOO_LARGE, d(4, 8, W.BF16, W.I8, "rmsnorm", **{ld: 1 << 60}))
+        refused(TOO_LARGE, d(1 << 39, 8, W.BF16, W.I8, "rmsnorm", **{ld: 1 << 39}))
     refused(TOO_LARGE, d(4, 1 << 31, W.BF16, W.I8))
-    refused(TOO_LARGE, d(1 << 40, 8, W.BF16, W.I8))
+    refused(TOO_LARGE, d(1 << 58, 8, W.BF16, W.I8))
     bad = d(4, 8, W.BF16, W.I8)
     bad.kind = 3
     refused(INVALID, bad)
@@ -76,6 +77,13 @@ def test_operands_that_are_refused():
     refused(INVALID, wide, residual=0x40000, sum_out=0x10000)
     wide = d(4, 8, W.BF16, W.I8, "rmsnorm", lds=16)
     refused(INVALID, wide, residual=0x40000, sum_out=0x40000)
+    # the outputs lie by themselves
+    refused(INVALID, plain, 0x10000, 0x10000)
+    refused(INVALID, plain, 0x10000, 0x20000, 0x10000)
+    refused(INVALID, plain, 0x10000, 0x20000, 0x20000)
+    refused(INVALID, norm, residual=0x20000)
+    refused(INVALID, norm, weight=0x30000)
+    refused(INVALID, norm, residual=0x40000, sum_out=0x20000)
     # gate and up side by side need rows of twice the width
     refused(INVALID, d(4, 8, W.BF16, W.I8, "silu_mul", ldx=15))
 
