@@ -497,6 +497,58 @@ __device__ __noinline__ void staged_rows_out(TC* C, void* const* peers, uint32_t
   }
 }
 
+// Whole staged rows (128 bytes each) to a C whose rows do not start on 16-byte boundaries.  Only the
+// integer kernels have these two: their mere presence cost the others' short-K shapes up to 10 %.
+// (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 63 us, 4096 x 4100 x 4096 98 -> 56 us,
+// fp32 C 4096 x 4097 x 4096 109 -> 69 us; with aligned rows 46 us.)
+// Rows on 4-byte boundaries: a row per step, a word per lane.
+__device__ __noinline__ void staged_rows_words(char* dst, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
+                                               uint32_t xor_mask) {
+#pragma unroll 4
+  for (uint32_t r = 0; r < n; ++r, dst += pitch) {
+    uint32_t w;
+    asm volatile("ld.shared.u32 %0, [%1];"
+                 : "=r"(w)
+                 : "r"(staged_chunk(stage, r, lane >> 2, xor_mask) + 4u * (lane & 3u))
+                 : "memory");
+    *reinterpret_cast<uint32_t*>(dst + 4u * lane) = w;
+  }
+}
+// Rows of 16-bit elements at any element: four rows per step in aligned 16-byte units, each put
+// together from the end of one lane's piece and the start of the next one's; the first and last unit
+// of a row, which the neighbouring chunks share, go element by element.
+__device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
+                                                uint32_t xor_mask) {
+  const uint32_t sub = lane >> 3, ch = lane & 7u;
+#pragma unroll 2
+  for (uint32_t it = 0; it < 8; ++it) {
+    const uint32_t rr = it * 4u + sub;
+    char* const dst = dst0 + (int64_t)rr * pitch;
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(dst) & 15u);
+    const uint4 piece = ld_shared_v4(staged_chunk(stage, rr, ch, xor_mask));
+    uint32_t v[8] = {__shfl_up_sync(0xffffffffu, piece.x, 1), __shfl_up_sync(0xffffffffu, piece.y, 1),
+                     __shfl_up_sync(0xffffffffu, piece.z, 1), __shfl_up_sync(0xffffffffu, piece.w, 1),
+                     piece.x, piece.y, piece.z, piece.w};
+    const uint32_t by = 16u - off;   // the unit starts `by` bytes into the two pieces (2 .. 16)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = by & 16u ? v[i + 4] : v[i];
+#pragma unroll
+    for (int i = 0; i < 6; ++i) v[i] = by & 8u ? v[i + 2] : v[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) v[i] = by & 4u ? v[i + 1] : v[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8u * (by & 3u));
+    if (rr >= n) continue;
+    if (ch > 0 || off == 0) *reinterpret_cast<uint4*>(dst - off + 16u * ch) = make_uint4(v[0], v[1], v[2], v[3]);
+    if (off) {
+      const uint32_t head = (16u - off) >> 1, tail = off >> 1;
+      if (ch < head) *reinterpret_cast<__half*>(dst + 2u * ch) = *staged_elem<__half>(stage, rr, ch, xor_mask);
+      if (ch < tail)
+        *reinterpret_cast<__half*>(dst + 2u * (64u - tail + ch)) = *staged_elem<__half>(stage, rr, 64u - tail + ch, xor_mask);
+    }
+  }
+}
+
 // One warp's 32 rows x NC columns of D = C (lane = row; NC * sizeof(TC) = 128 bytes): scale, add
 // the old C if asked, round once, fold the rounded values into `red` (the row fold sees what a
 // reduce of the stored C would see), and store:
@@ -508,7 +560,7 @@ __device__ __noinline__ void staged_rows_out(TC* C, void* const* peers, uint32_t
 //   direct: every thread writes its own row piece (16-byte stores at row stride);
 //   a C without 16-byte alignment, or the chunk that crosses the last column, goes element-wise.
 // `stage` is the warp's staging area (shared-memory address), `warp_row0` the D row of lane 0.
-template <typename TC, int NC>
+template <typename TC, int NC, bool kInt>
 __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint32_t stage,
                                                uint32_t lane, uint32_t warp_row0, uint32_t col0,
                                                const uint32_t (&acc)[NC], float& red) {
@@ -652,6 +704,12 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
           *reinterpret_cast<uint4*>(reinterpret_cast<TC*>(x.peers[q]) + off) = piece;
       }
     }
+  } else if (kInt && full && x.n_peers == 0) {
+    char* const dst = reinterpret_cast<char*>(C + (int64_t)warp_row0 * p.ldc + col0);
+    const int64_t pitch = p.ldc * (int64_t)sizeof(TC);
+    const uint32_t n = p.rows > warp_row0 ? min(32u, p.rows - warp_row0) : 0u;
+    if (((reinterpret_cast<uintptr_t>(dst) | (uintptr_t)pitch) & 3u) == 0) staged_rows_words(dst, pitch, n, stage, lane, xm);
+    else staged_rows_halves(dst, pitch, n, stage, lane, xm);
   } else {
     staged_rows_out<TC, NC>(C, x.peers, x.n_peers, p.ldc, p.rows, p.cols, stage, lane, warp_row0, col0, xm);
   }
@@ -667,13 +725,14 @@ __device__ __forceinline__ void epilogue_item(const EpiArgs& ep, EpiExt& ex, uin
                                               uint32_t cols_item, uint32_t t_row, float& red) {
   constexpr int CH = 128 / (int)sizeof(TC);
   for (uint32_t cc = 0; cc < cols_item; cc += CH) {
+    if (kInt && col0 + cc >= ep.cols) break;   // the rest of the item lies behind the last column
     uint32_t v[CH];
 #pragma unroll
     for (int h = 0; h < CH / 32; ++h)
       ptx::tmem_ld_32x32b_x32(t_row + cc + 32u * h, reinterpret_cast<uint32_t(&)[32]>(v[32 * h]));
     ptx::tmem_ld_wait();
     if constexpr (!std::is_same_v<TC, int32_t>) sums_to_f32<kInt>(v);
-    epilogue_chunk<TC, CH>(ep, ex, stage, lane, warp_row0, col0 + cc, v, red);
+    epilogue_chunk<TC, CH, kInt>(ep, ex, stage, lane, warp_row0, col0 + cc, v, red);
   }
 }
 

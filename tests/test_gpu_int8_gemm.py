@@ -140,6 +140,11 @@ PLANS = [
     (256, 512, 256, "tcgen05_pair", {}),
     (300, 520, 272, "tcgen05_pair", {}),                                 # ragged rows, columns and K
     (700, 1000, 4112, "tcgen05_pair", {"k_split": -1}),                  # many k-blocks, narrow last wave
+    (300, 521, 272, "tcgen05_pair", {}),                                 # rows of C at any element
+    (520, 1029, 300, "tcgen05_pair", {}),
+    (290, 518, 272, "tcgen05_pair", {"epilogue": 3}),
+    (333, 201, 400, "tcgen05", {"force_kernel": "tcgen05"}),
+    (333, 390, 400, "tcgen05", {"force_kernel": "tcgen05"}),
     (512, 768, 640, "tcgen05_pair", {"epilogue": 1}),
     (512, 768, 640, "tcgen05_pair", {"epilogue": 2}),
     (512, 768, 640, "tcgen05_pair", {"epilogue": 3}),
