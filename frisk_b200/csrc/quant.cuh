@@ -261,33 +261,39 @@ __device__ __forceinline__ void store8(T* p, const f2 (&f)[4]) {
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
-// Eight values into eight bytes.
-__device__ __forceinline__ uint2 encode8x8(const f2 (&v)[4], int qt) {
-  union {
-    uint32_t u[2];
-    uint16_t h[4];
-  } r;
+// A thread's NV groups of eight values into eight bytes each.
+template <int NV>
+__device__ __forceinline__ void encode_groups(const f2 (&v)[NV][4], int qt, uint2 (&out)[NV]) {
   if (qt == FRISK_DT_I8) {
     // v + 1.5 * 2^23 rounds v to the nearest integer, ties to even, and holds it in its low byte
     // (the conversion instruction shares its unit with the gate's 2^x and reciprocal)
-    uint32_t b[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f2 m = add2(v[j], pack2(12582912.f));
-      b[2 * j] = __float_as_uint(lo2(m));
-      b[2 * j + 1] = __float_as_uint(hi2(m));
+    for (int i = 0; i < NV; ++i) {
+      uint32_t b[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f2 m = add2(v[i][j], pack2(12582912.f));
+        b[2 * j] = __float_as_uint(lo2(m));
+        b[2 * j + 1] = __float_as_uint(hi2(m));
+      }
+      uint32_t* o = &out[i].x;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        o[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
     }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-      r.u[j] = __byte_perm(__byte_perm(b[4 * j], b[4 * j + 1], 0x0040), __byte_perm(b[4 * j + 2], b[4 * j + 3], 0x0040), 0x5410);
-  } else if (qt == FRISK_DT_E4M3) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[j]), hi2(v[j])), __NV_SATFINITE, __NV_E4M3);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r.h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[j]), hi2(v[j])), __NV_SATFINITE, __NV_E5M2);
+    return;
   }
-  return make_uint2(r.u[0], r.u[1]);
+  auto floats = [&](__nv_fp8_interpretation_t kind) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = __nv_cvt_float2_to_fp8x2(make_float2(lo2(v[i][j]), hi2(v[i][j])), __NV_SATFINITE, kind);
+      out[i] = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+  };
+  if (qt == FRISK_DT_E4M3) floats(__NV_E4M3);
+  else floats(__NV_E5M2);
 }
 
 // gate / (1 + exp(-gate)) * up for two elements.  e = exp(-gate) = 2^t, t = -gate log2(e): the product
@@ -443,10 +449,12 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   if (!live) return;
   divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+  uint2 bytes[NV];
+  encode_groups<NV>(g, p.q_type, bytes);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
-    if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = encode8x8(g[i], p.q_type);
+    if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = bytes[i];
   }
 }
 
@@ -656,12 +664,13 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
   row_fold<KIND>(sum, mx, s_sum, s_max, slot * wpr + warp_in_row, lane, slot, wpr);
   if (!live) return;
   divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  uint2 bytes[NV];
+  encode_groups<NV>(g, p.q_type, bytes);
   uint32_t qw[NV][2];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const uint2 b = encode8x8(g[i], p.q_type);
-    qw[i][0] = b.x;
-    qw[i][1] = b.y;
+    qw[i][0] = bytes[i].x;
+    qw[i][1] = bytes[i].y;
   }
   store_ragged<1, NV>(static_cast<unsigned char*>(p.q) + r * p.ldq, c0, cols, qw, lane);
 }
@@ -803,10 +812,12 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
     warp_fold<FRISK_QUANT_SILU_MUL>(sum, mx);
     divide<NV>(g, row_divisor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+    uint2 eight[NV];
+    encode_groups<NV>(g, p.q_type, eight);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int gidx = t + i * step;
-      if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * gidx) = encode8x8(g[i], p.q_type);
+      if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * gidx) = eight[i];
     }
     buf ^= 1;
     stage += teams;
