@@ -90,7 +90,9 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   const bool aligned = p.cols % 8 == 0 && rows_on(p.x, p.ldx, es, 16) && rows_on(p.other, p.ldo, es, 16) &&
                        rows_on(p.sum_out, p.lds, es, 16) && rows_on(p.q, p.ldq, 1, 8) && rows_on(p.weight, 0, 1, 16);
   constexpr int64_t kMaxCtas = 0x7fffffff;
-  if (p.cols > 8 * 1024 * kMaxGroups || p.rows > kMaxCtas) {   // more than registers hold, or than a grid
+  if (aligned && p.cols > 8 * 1024 * kMaxGroups)   // more than registers hold
+    return go(frisk_quant::quant_rows_wide_kernel<TIn, TW, KIND>, std::min(p.rows, kMaxCtas), dim3(1024), 0, p, st);
+  if (p.cols > 8 * 1024 * kMaxGroups || p.rows > kMaxCtas) {   // ... or rows than a grid has CTAs
     return go(frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND>, std::min(p.rows, kMaxCtas), dim3(256), 0, p, st);
   }
   const int64_t groups = ceil_div(p.cols, 8);

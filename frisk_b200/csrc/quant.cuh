@@ -458,6 +458,56 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   }
 }
 
+// Rows wider than a CTA's registers hold, with the alignment of quant_rows_kernel: two passes over the
+// row, the second one from L2, a group of eight per thread and step.  (h goes to sum_out in the second
+// pass: the first one may not yet have read its place.)
+template <typename TIn, typename TW, int KIND>
+__global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
+  __shared__ float s_sum[32];
+  __shared__ uint32_t s_max[32];
+  const int t = threadIdx.x, lane = t & 31, groups = (int)(p.cols >> 3);
+  const TW* w = static_cast<const TW*>(p.weight);
+  after_the_kernel_before();
+  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
+    const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
+    TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
+    f2 g[1][4], sums = 0;
+    float top = 0.f;
+    auto values = [&](int64_t c, bool store, f2& sq, float& mx) {
+      const Eight<TIn> ex = load8(x + c);
+      Eight<TIn> eo = ex;
+      if (KIND != FRISK_QUANT_PLAIN && o) eo = load8(o + c);
+      group_values<TIn, KIND>(
+          ex, eo, o != nullptr,
+          [&](f2 (&v)[4]) {
+            if (w) unpack8(load8_shared_by_rows(w + c), v);
+            return w != nullptr;
+          },
+          [&](const f2 (&h)[4]) {
+            if (store && so) store8(so + c, h);
+          },
+          g[0], sq, mx);
+    };
+#pragma unroll 2
+    for (int i = t; i < groups; i += 1024) values(8 * (int64_t)i, false, sums, top);
+    float sum = lo2(sums) + hi2(sums);
+    uint32_t mx = __float_as_uint(top);
+    row_fold<KIND>(sum, mx, s_sum, s_max, t >> 5, lane, 0, 32);
+    const float d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
+    uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+#pragma unroll 2
+    for (int i = t; i < groups; i += 1024) {
+      values(8 * (int64_t)i, true, sums, top);
+      divide<1>(g, d);
+      uint2 bytes[1];
+      encode_groups<1>(g, p.q_type, bytes);
+      *reinterpret_cast<uint2*>(q + 8 * (int64_t)i) = bytes[0];
+    }
+    __syncthreads();   // the shared arrays are written again by the next row
+  }
+}
+
 // ---- the same for rows at any alignment and width -----------------------------------------------
 // Memory is still touched in aligned words of 16 bytes (8 for q): a group that starts inside a word is
 // shifted together from the words it lies in, and a stored word from the end of one lane's group and

@@ -258,8 +258,9 @@ def test_captured_into_a_graph_and_on_another_stream():
 
 @pytest.mark.parametrize("q_type", [W.I8, W.E4M3], ids=ids)
 @pytest.mark.parametrize("rows,cols,in_type", [(600, 3080, W.BF16), (1500, 4096, W.F32), (1201, 3336, W.F16), (640, 8192, W.BF16),
-                                               (601, 16384, W.F32), (700, 16384, W.BF16)],
-                         ids=["600x3080", "1500x4096", "1201x3336", "640x8192", "601x16384", "700x16384"])
+                                               (601, 16384, W.F32), (700, 16384, W.BF16),
+                                               (400, 40000, W.BF16), (5, 53248, W.F32), (3, 40001, W.F16)],
+                         ids=["600x3080", "1500x4096", "1201x3336", "640x8192", "601x16384", "700x16384", "400x40000", "5x53248", "3x40001"])
 @pytest.mark.parametrize("kind", ["plain", "rmsnorm", "silu_mul"])
 def test_many_wide_rows(kind, rows, cols, in_type, q_type):
     many_rows(kind, rows, cols, in_type, q_type)
