@@ -531,20 +531,23 @@ __device__ __forceinline__ void shift_words(uint32_t (&v)[W + 4], uint32_t by) {
   for (int i = 0; i < W; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8u * (by & 3u));
 }
 
-// Elements c .. c + 7 of a row of a buffer that spans [lo, hi); zeros past the row's end.  A group that
-// crosses that end, or whose words reach out of the buffer, is read element by element.
+// Elements c .. c + 7 of a row; zeros past its end.  A group whose words reach out of the row is read
+// element by element: what lies there may be no part of any buffer, or another row that is being
+// replaced by its sum at that moment.
 template <typename T>
 struct Ragged {
   uint32_t w[2 * sizeof(T) + 4];
   uint32_t by;   // where the group starts in w
 };
 template <typename T>
-__device__ __forceinline__ void load8_ragged(Ragged<T>& g, const T* row, int c, int cols, const void* lo, const void* hi) {
+__device__ __forceinline__ void load8_ragged(Ragged<T>& g, const T* row, int c, int cols) {
   constexpr int W = 2 * sizeof(T);   // 32-bit words of a group
   const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
   g.by = (uint32_t)(at & 15u);
   const uint4* p = reinterpret_cast<const uint4*>(at - g.by);
-  if (c + 8 <= cols && p >= lo && p + W / 4 + 1 <= hi) {
+  // (elements in front of the group in its first word, and behind it in the last one)
+  const int before = (int)g.by / (int)sizeof(T), after = 16 / (int)sizeof(T) - before;
+  if (c >= before && c + 8 + after <= cols) {
 #pragma unroll
     for (int i = 0; i < W / 4 + 1; ++i) {
       asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -652,8 +655,6 @@ __device__ __forceinline__ void store_ragged(unsigned char* row, int c0, int col
   }
 }
 
-// (A word read at a row's edge may hold elements of the next row, which another CTA may be replacing
-// by its sum at that moment; they are shifted out.)
 template <typename TIn, typename TW, int KIND, int NV>
 __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params p) {
   __shared__ float s_sum[32];
@@ -663,11 +664,9 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
   const int64_t r = (int64_t)blockIdx.x * blockDim.y + slot;
   const bool live = r < p.rows;
   const int cols = live ? (int)p.cols : 0, c0 = warp_in_row * 256 * NV;   // the warp's first element
-  const TIn* x0 = static_cast<const TIn*>(p.x);
-  const TIn* o0 = static_cast<const TIn*>(p.other);
   const TW* w = static_cast<const TW*>(p.weight);
-  const TIn* x = x0 + r * p.ldx;
-  const TIn* o = o0 ? o0 + r * p.ldo : nullptr;
+  const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
+  const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
   const bool w_aligned = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
 
   after_the_kernel_before();
@@ -675,8 +674,8 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = c0 + 8 * (32 * i + lane);
-    load8_ragged(rx[i], x, c, cols, x0, x0 + (p.rows - 1) * p.ldx + p.cols);
-    if (KIND != FRISK_QUANT_PLAIN && o) load8_ragged(ro[i], o, c, cols, o0, o0 + (p.rows - 1) * p.ldo + p.cols);
+    load8_ragged(rx[i], x, c, cols);
+    if (KIND != FRISK_QUANT_PLAIN && o) load8_ragged(ro[i], o, c, cols);
   }
   f2 g[NV][4];
   f2 sums = 0;
@@ -694,7 +693,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
             unpack8(load8_shared_by_rows(w + c), v);
           } else if (w) {
             Ragged<TW> rw;
-            load8_ragged(rw, w, c, cols, w, w + p.cols);
+            load8_ragged(rw, w, c, cols);
             unpack8(take8(rw), v);
           }
           return w != nullptr;
