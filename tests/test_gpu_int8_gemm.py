@@ -203,7 +203,7 @@ def test_scales_and_result_types_on_every_plan(M, N, K, kernel, kw, ct, clear):
 
 
 @pytest.mark.parametrize("kind", ["max", "add", "min"])
-@pytest.mark.parametrize("M,N,K", [(300, 520, 272), (512, 768, 640)])
+@pytest.mark.parametrize("M,N,K", [(300, 520, 272), (512, 768, 640), (300, 521, 272), (130, 1030, 300)])
 def test_row_reduce_folded_into_the_epilogue(M, N, K, kind):
     a, b, sa, sb = make(M, N, K, 9)
     c, dst = np.zeros((M, N), np.uint16), np.zeros(M, np.uint16)
@@ -308,3 +308,27 @@ def test_misaligned_bases_still_give_the_right_answer():
     assert plan.refresh_info()["cuda_core_runs"] == 1
     plan.close()
     check(c.cpu().numpy(), *expect(a, b, sa, sb), W.F32)
+
+
+@pytest.mark.parametrize("N", [32768, 32761])
+def test_offsets_past_32_bits(N):
+    """More than 2^31 elements of C: the last rows."""
+    import torch
+    dev = torch.device("cuda:0")
+    M, K = 66000, 64
+    A = torch.zeros((M, K), dtype=torch.int8, device=dev)
+    pick = [0, 65535, 65536, M - 1]
+    a, b, sa, sb = make(len(pick), N, K, 15)
+    A[pick] = torch.from_numpy(a).to(dev)
+    B = torch.from_numpy(np.ascontiguousarray(b.T)).to(dev)
+    scale = torch.ones(M, device=dev)
+    scale[pick] = torch.from_numpy(sa).to(dev)
+    c = torch.full((M, N), 7.0, dtype=torch.bfloat16, device=dev)
+    plan = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True)
+    ws = torch.zeros(max(plan.workspace_bytes, 16), dtype=torch.uint8, device=dev)
+    plan.run(A, B, c, scale, torch.from_numpy(sb).to(dev), ws, stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    plan.close()
+    check(c[pick].view(torch.int16).cpu().numpy().view(np.uint16), *expect(a, b, sa, sb), W.BF16)
+    c[pick] = 0
+    assert not bool(c.any())

@@ -296,3 +296,70 @@ def many_rows(kind, rows, cols, in_type, q_type):
     check_q(q.cpu().numpy().view(W.storage_numpy_dtype(q_type)), s.cpu().numpy(), v, kind, q_type)
     if kind == "rmsnorm":
         check_sum(h.cpu().numpy().view(x.dtype), hw, in_type)
+
+
+@pytest.mark.parametrize("cols", [1000, 1001, 4096, 40000])
+@pytest.mark.parametrize("in_type", [W.F32, W.BF16], ids=ids)
+def test_many_rows_with_the_sum_in_place(in_type, cols):
+    """The sum over x, then over the residual, of many packed rows: what separate buffers give."""
+    import torch
+    dev = torch.device("cuda:0")
+    rows = 700 if cols < 40000 else 40
+    x, kw = inputs(rows, cols, in_type, "rmsnorm", 15)
+    on = lambda a: torch.from_numpy(np.ascontiguousarray(a).view(np.uint8)).to(dev)  # noqa: E731
+    weight, desc = on(kw["weight"]), R.quant_desc(rows, cols, in_type, W.E4M3, "rmsnorm")
+    got = []
+    for where in ("apart", "x", "residual"):
+        bx, br = on(x), on(kw["residual"])
+        h = torch.zeros_like(bx) if where == "apart" else bx if where == "x" else br
+        q, s = torch.zeros((rows, cols), dtype=torch.uint8, device=dev), torch.zeros(rows, device=dev)
+        R.quant_run(desc, bx, q, s, weight=weight, residual=br, sum_out=h)
+        torch.cuda.synchronize()
+        got.append((q, s, h))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert torch.equal(a, b)
+    v, h = ref.ref_quant(x, in_type, "rmsnorm", **kw)
+    check_q(got[0][0].cpu().numpy(), got[0][1].cpu().numpy(), v, "rmsnorm", W.E4M3)
+    check_sum(got[0][2].cpu().numpy().view(x.dtype).reshape(h.shape), h, in_type)
+
+
+def test_streamed_rows_captured_into_a_graph():
+    import torch
+    dev = torch.device("cuda:0")
+    rows, cols = 1200, 16384
+    desc = R.quant_desc(rows, cols, W.BF16, W.E4M3, "silu_mul")
+    x = torch.zeros((rows, 2 * cols), dtype=torch.bfloat16, device=dev)
+    q, s = torch.zeros((rows, cols), dtype=torch.uint8, device=dev), torch.zeros(rows, device=dev)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        R.quant_run(desc, x, q, s, stream=side.cuda_stream)
+    for seed in (1, 2):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(device=dev).manual_seed(seed), device=dev))
+        q2, s2 = torch.zeros_like(q), torch.zeros_like(s)
+        R.quant_run(desc, x, q2, s2, stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(q, q2) and torch.equal(s, s2) and bool((s > 0).all())
+
+
+@pytest.mark.parametrize("cols", [32768, 32761])
+def test_offsets_past_32_bits(cols):
+    """More than 2^31 elements (and 2^32 bytes) in x and more than 2^31 bytes in q: the last rows."""
+    import torch
+    dev = torch.device("cuda:0")
+    rows = 66000
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device=dev)
+    q = torch.full((rows, cols), 0x5A, dtype=torch.uint8, device=dev)
+    s = torch.zeros(rows, device=dev)
+    pick = [0, 1, 65535, 65536, rows - 2, rows - 1]
+    host, _ = inputs(len(pick), cols, W.BF16, "plain", 16)
+    x[pick] = torch.from_numpy(host.view(np.int16)).view(torch.bfloat16).to(dev)
+    R.quant_run(R.quant_desc(rows, cols, W.BF16, W.I8), x, q, s)
+    torch.cuda.synchronize()
+    v, _ = ref.ref_quant(host, W.BF16, "plain")
+    check_q(q[pick].cpu().numpy().view(np.int8), s[pick].cpu().numpy(), v, "plain", W.I8)
+    q[pick] = 0
+    assert not bool(q.any()) and int((s == 2.0 ** -126).sum()) == rows - len(pick)
