@@ -1428,7 +1428,10 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
     // Between 65 and 128 rows the few-row plan pays only in its cluster form (128 x 8192 x 8192:
     // 35 us against 59 us for whole tiles on 32 SMs); where clusters do not apply (few tiles, or
     // more tiles than SMs) whole tiles are as good or better (128 x 28672 x 4096: 45 against 79 us).
-    if (kind == FRISK_KERNEL_SKINNY && d.M > 64 && !d.force_kernel && pl->gp.split_mode != 3)
+    // int8 moves half the bytes a column, so there the wide shapes change over from 32 rows on
+    // (28672 x 4096: 32 rows 32.7 -> 27.6 us, 64 rows 38.6 -> 27.7; 24 rows 31.4 against 33.6).
+    const bool wide_i8 = d.a_type == FRISK_DT_I8 && d.M >= 32 && d.N > 128 * (int64_t)pl->sm_count && !d.num_ctas;
+    if (kind == FRISK_KERNEL_SKINNY && (d.M > 64 || wide_i8) && !d.force_kernel && pl->gp.split_mode != 3)
       plan_tcgen05(pl, /*swap=*/false, /*pair=*/false);
     // Few tiles of C against a long K: whole tiles would leave most SMs idle (512 x 512 x 65536:
     // 8 tiles; measured 227 us against 43 us for cuBLAS), so K is split over clusters or, where

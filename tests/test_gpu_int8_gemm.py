@@ -170,6 +170,10 @@ PLANS = [
     (16, 512, 4096, "skinny", {"force_kernel": "skinny"}),
     (33, 4100, 528, "skinny", {}),
     (64, 2048, 2048, "skinny", {}),
+    (31, 20000, 272, "skinny", {}),                                      # more columns than the SMs' tiles:
+    (32, 20000, 272, "tcgen05", {}),                                     # whole tiles from 32 rows on
+    (47, 19001, 528, "tcgen05", {}),
+    (32, 20000, 272, "skinny", {"num_ctas": 148}),
     (100, 8192, 512, "skinny", {}),
     (128, 8192, 1040, "skinny", {}),
     (16, 8192, 1024, "skinny", {"num_ctas": 97}),                        # stream-K: partials in slots

@@ -62,6 +62,7 @@ def test_builder_and_parser_take_8_bit_integers():
 def test_kernel_families_and_the_fixed_scratch_entry_point():
     for (M, N, K), kernel in (((8192, 8192, 8192), "tcgen05_pair"), ((16, 8192, 8192), "i8_rows"), ((1, 4096, 4096), "i8_rows"),
                               ((8, 8192, 8192), "i8_rows"), ((17, 8192, 8192), "skinny"),
+                              ((31, 28672, 4096), "skinny"), ((32, 28672, 4096), "tcgen05"), ((64, 8192, 8192), "skinny"),
                               ((128, 192, 256), "tcgen05")):
         p = R.GemmPlan(M, N, K, W.I8, W.BF16, transB=True, scales=True)
         assert p.info["kernel_name"] == kernel and p.info["tile_k"] == 128, p.info
