@@ -397,6 +397,9 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
     // percent of the SMs a cluster plan has to use: measured, 64 CTAs in clusters still beat
     // stream-K over all SMs (16x2048x2048: 10.4 against 15.5 us; 32x2048x8192: 18.7 against 25.7)
     uint32_t min_cover = 40;
+    // int8: any share (128 x 128 x 8192: stream-K over 28 CTAs 30.7 us, two clusters of eight 7.3;
+    // 64 x 256 x 4096 31.4 -> 5.6, 32 x 512 x 8192 31 -> 6.0)
+    if (d.a_type == FRISK_DT_I8) min_cover = 0;
 #ifdef FRISK_B200_MEASURE
     if (const char* e = getenv("FRISK_B200_MIN_COVER")) min_cover = (uint32_t)atoi(e);
 #endif
@@ -419,8 +422,9 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
         if (t * s * 100u >= (uint32_t)pl->sm_count * min_cover) cand[n_cand++] = Cand{t * s, mi, s};
       }
     }
-    std::sort(cand, cand + n_cand, [](const Cand& x, const Cand& y) {
-      return x.ctas != y.ctas ? x.ctas > y.ctas : x.mi > y.mi;
+    const bool low_first = d.a_type == FRISK_DT_I8 && !swap;   // (2048 x 64 x 4096 9.5 -> 8.3 us)
+    std::sort(cand, cand + n_cand, [low_first](const Cand& x, const Cand& y) {
+      return x.ctas != y.ctas ? x.ctas > y.ctas : (x.mi > y.mi) != low_first;
     });
     use_cluster = cluster_try >= 0 && cluster_try < n_cand && d.num_ctas == 0;
     if (use_cluster) {
@@ -1470,24 +1474,43 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
       // With four tiles or fewer the single-CTA clusters below stay ahead (256 x 256 x 4096: 9.0
       // against 11.5 us).  Clusters of eight CTAs with 214 KB of shared memory each are placed
       // about a dozen at a time, which is why larger problems get two pairs per cluster.
-      const bool deep = force_split || (few ? kbs >= 48 : kbs >= 192);
+      bool deep = force_split || (few ? kbs >= 48 : kbs >= 192);
       const uint64_t tiles128 = (uint64_t)((d.M + 255) / 256) * (uint64_t)((d.N + 127) / 128);
       const int whole_kernel = pl->info.kernel;
       const int64_t rows_pad = (d.M + 255) / 256 * 256, cols_pad = (d.N + 127) / 128 * 128;
       const bool full_tiles = 4 * (rows_pad - d.M) <= rows_pad && 4 * (cols_pad - d.N) <= cols_pad;
       int pcl = 0;
-      if (d.k_split == 3) {   // forced: four pairs per cluster where the SMs allow, else two
+      // int8, C of at most 32 tiles of 128 x 64: clusters of single CTAs come first where measured ahead,
+      // whole tiles / pair clusters -> single-CTA clusters, bf16 C unless stated:
+      //   up to 15 tiles (eight CTAs a cluster; C up to 64 wide from 16 k-blocks on): 256 x 256 x 1024 6.2 -> 5.4 us,
+      //     x 4096 9.6 -> 6.3, x 16384 13.4 -> 9.8; 1024 x 64 x 1024 4.7 -> 5.2;
+      //   more: from 32 k-blocks on 512 x 512 x 4096 10.9 -> 8.4 us, 160 x 512 x 4096 9.6 -> 8.6, x 2048 7.2 -> 8.1;
+      //     fp32 C from 16 on (512 x 512 x 2048 8.5 -> 7.4), C rows off the 16-byte grid from 8 on
+      //     (500 x 500 x 1024 14.1 -> 6.8); up to 128 unless 15 tiles of 128 x 128 hold C
+      //     (768 x 256 x 16384 14.3 -> 12.3, 512 x 512 x 16384 14.9 -> 15.3).
+      const bool c_rows = (d.ldc * elem_size(d.c_type)) % 16 == 0;
+      bool i8_split = false;
+      if (d.a_type == FRISK_DT_I8 && d.k_split == 0) {
+        const int64_t wide_tiles = ((d.M + 127) / 128) * ((d.N + 127) / 128);
+        i8_split = t128 <= 15 ? kbs >= (d.N > 64 ? 8u : 16u)
+                              : t128 <= 32 && kbs >= (!c_rows ? 8u : d.c_type == FRISK_DT_F32 ? 16u : 32u) &&
+                                    (kbs < 128 || wide_tiles <= 15);
+        deep = deep || i8_split;
+      }
+      if (i8_split) {   // below
+      } else if (d.k_split == 3) {   // forced: four pairs per cluster where the SMs allow, else two
         for (int sp : {4, 2})
           if (!pcl && pair_ok && tiles128 * 2 * sp <= (uint64_t)pl->sm_count && kbs >= 8u * sp) pcl = sp;
       } else if (d.k_split == 0 && pair_ok && d.a_type == FRISK_DT_I8 && kbs <= 128) {
         // Integers, measured again (their k-blocks are twice as deep): C rows off the 16-byte grid leave
-        // this kernel element by element (700 x 300 x 8192, bf16 C: 21.2 us, single-CTA clusters 11.7),
-        // and from twelve tiles on up to 45 % of padding rows pay (333 x 1000 x 8192 17.8 -> 13.3 us,
-        // 300 x 1000 x 8192 17.8 -> 13.3; 129 x 1000 x 8192, half padding, 10.8 -> 12.2: left out).
-        const bool c_rows = (d.ldc * elem_size(d.c_type)) % 16 == 0;
+        // this kernel element by element (700 x 300 x 8192, bf16 C: 21.2 us, single-CTA clusters 11.7);
+        // up to 45 % of padding rows pay from twelve tiles on (333 x 1000 x 8192 17.8 -> 13.3 us,
+        // 300 x 1000 x 8192 17.8 -> 13.3; 129 x 1000 x 8192, half padding, 10.8 -> 12.2: left out); four pairs per
+        // cluster up to fifteen tiles (1280 x 256 x 16384 18.6 -> 16.6, 640 x 640 x 16384 18.0 -> 15.9); nothing
+        // below 48 k-blocks (256 x 1152 x 4096 9.8 whole, 11.0 here).
         const bool padded = 20 * (rows_pad - d.M) <= 9 * rows_pad && 4 * (cols_pad - d.N) <= cols_pad;
-        if (c_rows && full_tiles && tiles128 >= 6 && tiles128 <= 9 && kbs >= 32) pcl = 4;
-        else if (c_rows && padded && tiles128 >= 12 && tiles128 * 4 <= (uint64_t)pl->sm_count && kbs >= 48) pcl = 2;
+        if (c_rows && padded && kbs >= 48 && tiles128 >= 6)
+          pcl = tiles128 <= 15 && (full_tiles || tiles128 >= 12) ? 4 : tiles128 >= 12 && tiles128 * 4 <= (uint64_t)pl->sm_count ? 2 : 0;
       } else if (d.k_split == 0 && pair_ok && full_tiles && kbs <= 128) {
         if (tiles128 >= 6 && tiles128 <= 9 && kbs >= 32) pcl = 4;
         else if (tiles128 >= 12 && tiles128 * 4 <= (uint64_t)pl->sm_count && kbs >= 48) pcl = 2;
@@ -1496,7 +1519,7 @@ int frisk_b200_gemm_plan_create(const frisk_gemm_desc* desc, frisk_gemm_plan** o
       if (pcl) {
         plan_tcgen05(pl, /*swap=*/false, /*pair=*/true, 0, false, 0, pcl);
         took_pcl = !pl->plan_error && (!pl->have_device || pair_clusters_fit(pl));
-        if (!took_pcl && d.k_split == 3 && pcl == 4) {   // forced: two pairs per cluster will do
+        if (!took_pcl && (d.k_split == 3 || (d.a_type == FRISK_DT_I8 && tiles128 >= 10)) && pcl == 4) {   // two pairs per cluster will do
           plan_tcgen05(pl, /*swap=*/false, /*pair=*/true, 0, false, 0, 2);
           took_pcl = !pl->plan_error && (!pl->have_device || pair_clusters_fit(pl));
         }

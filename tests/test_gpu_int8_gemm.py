@@ -178,6 +178,28 @@ PLANS = [
     (128, 8192, 1040, "skinny", {}),
     (16, 8192, 1024, "skinny", {"num_ctas": 97}),                        # stream-K: partials in slots
     (24, 512, 8192, "skinny", {"num_ctas": 148}),                        # more partials of a tile than its list holds
+    (17, 256, 144, "skinny", {}),                                        # one or two tiles: a cluster all the same,
+    (64, 256, 1168, "skinny", {}),                                       # with a part of K that is shorter or empty
+    (32, 512, 8192, "skinny", {}),
+    (128, 300, 1040, "skinny", {}),
+    (128, 128, 1152, "tcgen05", {}),                                     # small C: K over clusters of eight
+    (128, 128, 16384, "tcgen05", {}),
+    (40, 64, 2064, "tcgen05", {}),
+    (100, 200, 1100, "tcgen05", {}),
+    (130, 60, 2200, "tcgen05", {}),
+    (384, 320, 1024, "tcgen05", {}),
+    (160, 512, 4112, "tcgen05", {}),
+    (500, 500, 4112, "tcgen05", {}),
+    (499, 501, 1040, "tcgen05", {}),
+    (2048, 64, 4112, "tcgen05", {}),
+    (300, 640, 16400, "tcgen05", {}),
+    (1280, 256, 6160, "tcgen05_pair", {}),                               # four pairs to a cluster
+    (640, 640, 6144, "tcgen05_pair", {}),
+    (333, 1000, 6200, "tcgen05_pair", {}),
+    (600, 2008, 272, "tcgen05_pair", {"epilogue": 2}),                   # the last columns' chunk: on the 16-byte grid,
+    (600, 2004, 272, "tcgen05_pair", {}),                                # words, elements
+    (600, 2001, 272, "tcgen05_pair", {}),
+    (47, 19010, 144, "tcgen05", {}),
     (512, 512, 4096, "tcgen05_pair", {"k_split": 3}),                    # K over the pairs of a cluster
     (260, 128, 8192, "tcgen05_pair", {"k_split": 3}),
     (512, 500, 4096, "tcgen05_pair", {"k_split": 2}),                    # K planes
