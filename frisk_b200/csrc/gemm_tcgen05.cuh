@@ -499,12 +499,14 @@ __device__ __noinline__ void staged_rows_out(TC* C, void* const* peers, uint32_t
 
 // Whole staged rows (128 bytes each) to a C whose rows do not start on 16-byte boundaries.  Only the
 // integer kernels have these two: their mere presence cost the others' short-K shapes up to 10 %.
-// (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 63 us, 4096 x 4100 x 4096 98 -> 56 us,
-// fp32 C 4096 x 4097 x 4096 109 -> 69 us; with aligned rows 46 us.)
-// Rows on 4-byte boundaries: a row per step, a word per lane.
+// (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 53 us, 4096 x 4100 x 4096 98 -> 51 us,
+// fp32 C 4096 x 4097 x 4096 109 -> 61 us; with aligned rows 46 us.)
+// A row per step, a word per lane (bf16 C 7252 x 14645 x 160: four, eight, sixteen rows in flight 229, 199, 172 us;
+// in 16-byte units, with the selects that shifting those takes, 262).
+// Rows on 4-byte boundaries.
 __device__ __noinline__ void staged_rows_words(char* dst, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
                                                uint32_t xor_mask) {
-#pragma unroll 4
+#pragma unroll 16
   for (uint32_t r = 0; r < n; ++r, dst += pitch) {
     uint32_t w;
     asm volatile("ld.shared.u32 %0, [%1];"
@@ -514,38 +516,27 @@ __device__ __noinline__ void staged_rows_words(char* dst, int64_t pitch, uint32_
     *reinterpret_cast<uint32_t*>(dst + 4u * lane) = w;
   }
 }
-// Rows of 16-bit elements at any element: four rows per step in aligned 16-byte units, each put
-// together from the end of one lane's piece and the start of the next one's; the first and last unit
-// of a row, which the neighbouring chunks share, go element by element.
+// Rows of 16-bit elements at any element: the words of a row off the 4-byte grid are put together from
+// two lanes'; such a row's first and last element go by themselves.
 __device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
                                                 uint32_t xor_mask) {
-  const uint32_t sub = lane >> 3, ch = lane & 7u;
-#pragma unroll 2
-  for (uint32_t it = 0; it < 8; ++it) {
-    const uint32_t rr = it * 4u + sub;
-    char* const dst = dst0 + (int64_t)rr * pitch;
-    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(dst) & 15u);
-    const uint4 piece = ld_shared_v4(staged_chunk(stage, rr, ch, xor_mask));
-    uint32_t v[8] = {__shfl_up_sync(0xffffffffu, piece.x, 1), __shfl_up_sync(0xffffffffu, piece.y, 1),
-                     __shfl_up_sync(0xffffffffu, piece.z, 1), __shfl_up_sync(0xffffffffu, piece.w, 1),
-                     piece.x, piece.y, piece.z, piece.w};
-    const uint32_t by = 16u - off;   // the unit starts `by` bytes into the two pieces (2 .. 16)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = by & 16u ? v[i + 4] : v[i];
-#pragma unroll
-    for (int i = 0; i < 6; ++i) v[i] = by & 8u ? v[i + 2] : v[i];
-#pragma unroll
-    for (int i = 0; i < 5; ++i) v[i] = by & 4u ? v[i + 1] : v[i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __funnelshift_r(v[i], v[i + 1], 8u * (by & 3u));
-    if (rr >= n) continue;
-    if (ch > 0 || off == 0) *reinterpret_cast<uint4*>(dst - off + 16u * ch) = make_uint4(v[0], v[1], v[2], v[3]);
-    if (off) {
-      const uint32_t head = (16u - off) >> 1, tail = off >> 1;
-      if (ch < head) *reinterpret_cast<__half*>(dst + 2u * ch) = *staged_elem<__half>(stage, rr, ch, xor_mask);
-      if (ch < tail)
-        *reinterpret_cast<__half*>(dst + 2u * (64u - tail + ch)) = *staged_elem<__half>(stage, rr, 64u - tail + ch, xor_mask);
-    }
+  char* dst = dst0;
+#pragma unroll 16
+  for (uint32_t r = 0; r < n; ++r, dst += pitch) {
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(dst) & 2u);   // warp-uniform
+    uint32_t w;
+    asm volatile("ld.shared.u32 %0, [%1];"
+                 : "=r"(w)
+                 : "r"(staged_chunk(stage, r, lane >> 2, xor_mask) + 4u * (lane & 3u))
+                 : "memory");
+    const uint32_t before = __shfl_up_sync(0xffffffffu, w, 1);
+    if (off) w = __byte_perm(before, w, 0x5432);
+    if (!off || lane) *reinterpret_cast<uint32_t*>(dst - off + 4u * lane) = w;
+  }
+  dst = dst0 + (int64_t)lane * pitch;
+  if (lane < n && (reinterpret_cast<uintptr_t>(dst) & 2u)) {
+    *reinterpret_cast<__half*>(dst) = *staged_elem<__half>(stage, lane, 0, xor_mask);
+    *reinterpret_cast<__half*>(dst + 126) = *staged_elem<__half>(stage, lane, 63, xor_mask);
   }
 }
 
