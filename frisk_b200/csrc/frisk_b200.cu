@@ -493,7 +493,9 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
   // The area is reserved either way: the element-wise path of a C without 16-byte alignment goes
   // through it too.
   // desc.epilogue = 4 on a CTA-pair plan: TMA tensor stores out of two staging buffers per warp
-  // (needs rows of C that start on 16-byte boundaries, like every tensor map).
+  // (needs rows of C that start on 16-byte boundaries, like every tensor map, and that end on them: the
+  // hardware clips a store at 16-byte units, so of a row of 2037 bf16 elements at a pitch of 2040 it would
+  // write the three elements of padding too).
   // Taken by default when K is short (at most 32 k-blocks): the epilogue of a tile then takes
   // longer than its main loop, and the tensor stores need a fraction of the instructions
   // (measured, bf16 8192 x 8192 x K: K = 256 58.6 -> 41.4 us, K = 512 65.3 -> 54.3 us, equal from
@@ -505,7 +507,7 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
                                     (int64_t)(d.num_ctas > 1 ? std::min(d.num_ctas, pl->sm_count) : pl->sm_count);
   const bool want_tma = d.epilogue == 4 || (d.epilogue == 0 && (short_k || one_wave));
   const bool epi_tma = pair && !planes && !pcl && !pl->tf32 && want_tma &&
-                       (d.ldc * (int64_t)elem_size(d.c_type)) % 16 == 0;
+                       (d.ldc * (int64_t)elem_size(d.c_type)) % 16 == 0 && (d.N * (int64_t)elem_size(d.c_type)) % 16 == 0;
   const size_t epi_bytes = (split || pcl) ? 0 : (epi_tma ? 2 : 1) * frisk::kEpiStageBytes;
   // (the other pairs' images of the rows a CTA owns: [pair][row of the share][tile_n + 4] fp32)
   if (pcl) red_bytes = ((size_t)(pair_cluster - 1) * (128 / pair_cluster) * (g.tile_n + 4) * sizeof(float) + 1023) / 1024 * 1024;
