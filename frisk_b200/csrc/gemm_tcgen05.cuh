@@ -499,9 +499,9 @@ __device__ __noinline__ void staged_rows_out(TC* C, void* const* peers, uint32_t
 
 // Whole staged rows (128 bytes each) to a C whose rows do not start on 16-byte boundaries.  Only the
 // integer kernels have these two: their mere presence cost the others' short-K shapes up to 10 %.
-// (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 53 us, 4096 x 4100 x 4096 98 -> 51 us,
+// (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 52 us, 4096 x 4100 x 4096 98 -> 51 us,
 // fp32 C 4096 x 4097 x 4096 109 -> 61 us; with aligned rows 46 us.)
-// A row per step, a word per lane (bf16 C 7252 x 14645 x 160: four, eight, sixteen rows in flight 229, 199, 172 us;
+// A row per step, a word per lane (bf16 C 7252 x 14645 x 160: four, eight, sixteen rows in flight 229, 199, 161 us;
 // in 16-byte units, with the selects that shifting those takes, 262).
 // Rows on 4-byte boundaries.
 __device__ __noinline__ void staged_rows_words(char* dst, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
@@ -516,11 +516,13 @@ __device__ __noinline__ void staged_rows_words(char* dst, int64_t pitch, uint32_
     *reinterpret_cast<uint32_t*>(dst + 4u * lane) = w;
   }
 }
-// Rows of 16-bit elements at any element: the words of a row off the 4-byte grid are put together from
-// two lanes'; such a row's first and last element go by themselves.
-__device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint32_t n, uint32_t stage, uint32_t lane,
-                                                uint32_t xor_mask) {
+// Rows of 16-bit elements at any element, the first `nb` bytes of each (128 unless the chunk crosses the last
+// column): the words of a row off the 4-byte grid are put together from two lanes', an element that is left
+// at either end goes by itself (197 x 2037 x 176, the last chunk element by element 13.9 us, here 10.2).
+__device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint32_t n, uint32_t nb, uint32_t stage,
+                                                uint32_t lane, uint32_t xor_mask) {
   char* dst = dst0;
+  const bool on = 4u * lane + 4u <= nb, shifted = lane > 0 && 4u * lane + 2u <= nb;   // the lane's word is whole
 #pragma unroll 16
   for (uint32_t r = 0; r < n; ++r, dst += pitch) {
     const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(dst) & 2u);   // warp-uniform
@@ -531,13 +533,16 @@ __device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint3
                  : "memory");
     const uint32_t before = __shfl_up_sync(0xffffffffu, w, 1);
     if (off) w = __byte_perm(before, w, 0x5432);
-    if (!off || lane) *reinterpret_cast<uint32_t*>(dst - off + 4u * lane) = w;
+    // (predicated by hand: as a branch the rows go one after the other, 161 -> 232 us on the shape above)
+    asm volatile("{ .reg .pred p; setp.ne.u32 p, %2, 0; @p st.global.u32 [%0], %1; }" ::"l"(__cvta_generic_to_global(dst - off + 4u * lane)), "r"(w),
+                 "r"((uint32_t)(off ? shifted : on))
+                 : "memory");
   }
   dst = dst0 + (int64_t)lane * pitch;
-  if (lane < n && (reinterpret_cast<uintptr_t>(dst) & 2u)) {
-    *reinterpret_cast<__half*>(dst) = *staged_elem<__half>(stage, lane, 0, xor_mask);
-    *reinterpret_cast<__half*>(dst + 126) = *staged_elem<__half>(stage, lane, 63, xor_mask);
-  }
+  const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(dst) & 2u);
+  if (lane < n && off) *reinterpret_cast<__half*>(dst) = *staged_elem<__half>(stage, lane, 0, xor_mask);
+  if (lane < n && ((nb + off) & 2u))
+    *reinterpret_cast<__half*>(dst + nb - 2u) = *staged_elem<__half>(stage, lane, nb / 2u - 1u, xor_mask);
 }
 
 // One warp's 32 rows x NC columns of D = C (lane = row; NC * sizeof(TC) = 128 bytes): scale, add
@@ -695,12 +700,13 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
           *reinterpret_cast<uint4*>(reinterpret_cast<TC*>(x.peers[q]) + off) = piece;
       }
     }
-  } else if (kInt && full && x.n_peers == 0) {
+  } else if (kInt && x.n_peers == 0) {
     char* const dst = reinterpret_cast<char*>(C + (int64_t)warp_row0 * p.ldc + col0);
     const int64_t pitch = p.ldc * (int64_t)sizeof(TC);
     const uint32_t n = p.rows > warp_row0 ? min(32u, p.rows - warp_row0) : 0u;
-    if (((reinterpret_cast<uintptr_t>(dst) | (uintptr_t)pitch) & 3u) == 0) staged_rows_words(dst, pitch, n, stage, lane, xm);
-    else staged_rows_halves(dst, pitch, n, stage, lane, xm);
+    const uint32_t nb = (full ? (uint32_t)NC : p.cols - col0) * (uint32_t)sizeof(TC);
+    if (full && ((reinterpret_cast<uintptr_t>(dst) | (uintptr_t)pitch) & 3u) == 0) staged_rows_words(dst, pitch, n, stage, lane, xm);
+    else staged_rows_halves(dst, pitch, n, nb, stage, lane, xm);
   } else {
     staged_rows_out<TC, NC>(C, x.peers, x.n_peers, p.ldc, p.rows, p.cols, stage, lane, warp_row0, col0, xm);
   }

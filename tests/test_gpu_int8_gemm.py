@@ -247,22 +247,24 @@ def test_stays_inside_c_and_the_workspace():
     import torch
     dev = torch.device("cuda:0")
     for M, N, K, kw in ((1, 300, 144, {}), (16, 8192, 1024, {"num_ctas": 97}), (130, 257, 272, {}), (512, 500, 4096, {"k_split": 2}),
-                        (300, 520, 4099, {})):
+                        (300, 520, 4099, {}), (600, 2037, 176, {}), (300, 1025, 144, {}), (300, 1983, 144, {}), (47, 19010, 144, {}),
+                        (32, 512, 1168, {}), (100, 200, 1100, {})):
         a, b, sa, sb = make(M, N, K, 10)
-        for ct, ldc in ((W.BF16, N + 3), (W.F32, N + 4)):
+        for ct, ldc, shift in ((W.BF16, N + 3, 0), (W.BF16, N + 1, 2), (W.F16, N + 2, 6), (W.BF16, N + 8, 16), (W.F32, N + 4, 0),
+                               (W.F32, N + 1, 4)):
             es = W.ELEM_SIZE[ct]
             plan = R.GemmPlan(M, N, K, W.I8, ct, transB=True, scales=True, ldc=ldc, **kw)
-            guard = 256
+            guard = 256 + shift
             cbuf = torch.full((M * ldc * es + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
-            wbuf = torch.full((plan.workspace_bytes + 2 * guard,), 0x5A, dtype=torch.uint8, device=dev)
+            wbuf = torch.full((plan.workspace_bytes + 512,), 0x5A, dtype=torch.uint8, device=dev)
             A, B = torch.from_numpy(a).to(dev), torch.from_numpy(np.ascontiguousarray(b.T)).to(dev)
             dsa, dsb = torch.from_numpy(sa).to(dev), torch.from_numpy(sb).to(dev)
-            plan.run(A, B, cbuf.data_ptr() + guard, dsa, dsb, wbuf[guard:guard + plan.workspace_bytes] if plan.workspace_bytes else None,
+            plan.run(A, B, cbuf.data_ptr() + guard, dsa, dsb, wbuf[256:256 + plan.workspace_bytes] if plan.workspace_bytes else None,
                      stream=torch.cuda.current_stream().cuda_stream)
             torch.cuda.synchronize()
             host, ws = cbuf.cpu().numpy(), wbuf.cpu().numpy()
             assert (host[:guard] == 0x5A).all() and (host[guard + M * ldc * es:] == 0x5A).all()
-            assert (ws[:guard] == 0x5A).all() and (ws[guard + plan.workspace_bytes:] == 0x5A).all()
+            assert (ws[:256] == 0x5A).all() and (ws[256 + plan.workspace_bytes:] == 0x5A).all()
             rows = host[guard:guard + M * ldc * es].reshape(M, ldc * es)
             assert (rows[:, N * es:] == 0x5A).all()
             check(np.ascontiguousarray(rows[:, :N * es]).view(W.storage_numpy_dtype(ct)), *expect(a, b, sa, sb), ct)
