@@ -889,13 +889,25 @@ struct RepackJob {
 };
 constexpr int kRepackSeg = 2048;   // a warp's piece: four 16-byte chunks per lane
 
+// Sixteen bytes at an aligned address, of which only those inside [lo, hi) are read.
+__device__ __forceinline__ uint4 load16_inside(const unsigned char* p, const unsigned char* lo, const unsigned char* hi) {
+  if (p >= lo && p + 16 <= hi) return *reinterpret_cast<const uint4*>(p);
+  uint32_t x[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 16; ++e)
+    if (p + e >= lo && p + e < hi) x[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // Both operands of a gemm in one launch (jobs without rows are empty); a warp per piece of a row.
-// Sixteen bytes of the destination come out of five aligned words of the source, shifted together;
-// only pieces at the ends of a row or of the buffer go byte by byte, so that nothing outside the
-// buffer is read.
+// The lanes load the aligned 16 bytes that their piece begins in, take the next lane's from it, and shift the two
+// together by the row's offset; only at the ends of the buffer bytes are read one by one, so that nothing
+// outside it is.  (With the product, five words a lane shifted together -> here: 14 x 13233 x 1273 18.5 -> 15.2 us,
+// 215 x 1459 x 12923 31.7 -> 28.3, 333 x 1000 x 4099 15.9 -> 15.5, 655 x 3673 x 166 16.9 -> 17.2.)
 __global__ void __launch_bounds__(256) repack_rows_kernel(const RepackJob a, const RepackJob b) {
   frisk::ptx::griddep_launch_dependents();
   frisk::ptx::griddep_wait();
+  constexpr int U = kRepackSeg / 512;
   const int lane = threadIdx.x & 31;
   const int64_t items_a = a.rows * a.segs, items = items_a + b.rows * b.segs;
   for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += (int64_t)gridDim.x * 8) {
@@ -904,38 +916,45 @@ __global__ void __launch_bounds__(256) repack_rows_kernel(const RepackJob a, con
     const int64_t r = j.segs == 1 ? k : k / j.segs;
     const int64_t c0 = (k - r * j.segs) * kRepackSeg;
     const unsigned char* end = j.src + (j.rows - 1) * j.src_pitch + j.row_bytes;   // of the buffer
-    uint4 v[kRepackSeg / 512];
+    const unsigned char* row = j.src + r * j.src_pitch;
+    const uint32_t s = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);          // warp-uniform
+    const unsigned char* p = row + c0 - s + 16 * lane;
+    uint4 v[U + 1];
 #pragma unroll
-    for (int u = 0; u < kRepackSeg / 512; ++u) {
-      const int64_t c = c0 + (u * 32 + lane) * 16;
+    for (int u = 0; u <= U; ++u) {
       v[u] = make_uint4(0, 0, 0, 0);
-      if (c >= j.row_bytes) continue;
-      const unsigned char* p = j.src + r * j.src_pitch + c;
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)3);
-      const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(p) & 3) * 8u;
-      const bool whole = j.row_bytes - c >= 16;
-      if (whole && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-        v[u] = *reinterpret_cast<const uint4*>(p);
-      } else if (whole && reinterpret_cast<const unsigned char*>(w) >= j.src &&
-                 reinterpret_cast<const unsigned char*>(w + 5) <= end) {
-        const uint32_t w0 = w[0], w1 = w[1], w2 = w[2], w3 = w[3], w4 = w[4];
-        v[u].x = __funnelshift_r(w0, w1, sh);
-        v[u].y = __funnelshift_r(w1, w2, sh);
-        v[u].z = __funnelshift_r(w2, w3, sh);
-        v[u].w = __funnelshift_r(w3, w4, sh);
-      } else {
-        const int n = (int)(whole ? 16 : j.row_bytes - c);
-        uint32_t x[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (e < n) x[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
-        v[u] = make_uint4(x[0], x[1], x[2], x[3]);
-      }
+      const unsigned char* q = p + 512 * u;
+      if ((u == U && lane) || q >= row + j.row_bytes) continue;
+      v[u] = load16_inside(q, j.src, end);
     }
 #pragma unroll
-    for (int u = 0; u < kRepackSeg / 512; ++u) {
+    for (int u = 0; u < U; ++u) {
+      if (c0 + 512 * u >= j.dst_pitch) break;
       const int64_t c = c0 + (u * 32 + lane) * 16;
-      if (c < j.dst_pitch) *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = v[u];
+      uint32_t w[8] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      if (s) {
+        const uint4 give = lane ? v[u] : v[u + 1];
+        const int from = (lane + 1) & 31;
+        w[4] = __shfl_sync(0xffffffffu, give.x, from);
+        w[5] = __shfl_sync(0xffffffffu, give.y, from);
+        w[6] = __shfl_sync(0xffffffffu, give.z, from);
+        w[7] = __shfl_sync(0xffffffffu, give.w, from);
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = s & 8u ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = s & 4u ? w[i + 1] : w[i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 8u * (s & 3u));
+      }
+      if (c >= j.dst_pitch) continue;
+      if (c + 16 > j.row_bytes) {   // zeros behind the end of the row
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t n = j.row_bytes - c - 4 * i;
+          w[i] = n >= 4 ? w[i] : n <= 0 ? 0u : w[i] & (0xffffffffu >> (8 * (4 - (int)n)));
+        }
+      }
+      *reinterpret_cast<uint4*>(j.dst + r * j.dst_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
 }
