@@ -107,6 +107,19 @@ def test_the_longest_sums_do_not_overflow():
     assert np.array_equal(c, (a.astype(np.int64) @ b.astype(np.int64)).astype(np.float32))
 
 
+@pytest.mark.parametrize("M,N", [(64, 256), (128, 128), (20, 64), (200, 300), (640, 640)])
+def test_the_longest_sums_split_over_clusters(M, N):
+    K = 131071
+    a, b, _, _ = make(M, N, K, 16, full=True)
+    a[0], b[:, 0] = -128, -128
+    a[-1], b[:, -1] = 127, -128
+    c = np.zeros((M, N), np.float32)
+    plan = R.GemmPlan(M, N, K, W.I8, W.F32, transB=True)
+    plan.run_host(a, np.ascontiguousarray(b.T), c)
+    plan.close()
+    assert np.array_equal(c, np.rint(a.astype(np.float64) @ b.astype(np.float64)).astype(np.float32))
+
+
 def test_through_the_ir_builder():
     import frisk as F
     M, N, K = 200, 300, 160
