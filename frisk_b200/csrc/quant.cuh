@@ -83,29 +83,39 @@ __device__ __forceinline__ void warp_fold(float& sum, uint32_t& mx) {
 
 __device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 
+// What a row's elements are divided by: q = round(v * up / d).
+struct Divisor {
+  float d, up;
+};
+
 // scale[r] and the divisor of g from the row's sum of h^2 and maximum of |g| (as bits).  Every thread
 // of the row needs the divisor; the scale, with its root, only the one that stores it (`writer`).
 template <int KIND>
-__device__ __forceinline__ float row_divisor(float sum_sq, uint32_t max_bits, int64_t cols, float eps, int qt,
-                                             bool writer, float* scale) {
-  const float d = __fdiv_rn(__uint_as_float(max_bits), q_max(qt));
+__device__ __forceinline__ Divisor row_divisor(float sum_sq, uint32_t max_bits, int64_t cols, float eps, int qt,
+                                               bool writer, float* scale) {
+  const float top = __uint_as_float(max_bits);
   if (KIND != FRISK_QUANT_RMSNORM) {
+    const float d = __fdiv_rn(top, q_max(qt));
     const float s = max_bits > 0x7f800000u ? d : fmaxf(d, kTinyScale);
     if (writer) *scale = s;
-    return s;
+    return {s, 1.f};
   }
+  // A row of very small g: its maximum over Q would be a subnormal number of a few bits, so the row is
+  // worked on 2^96 times as large (exact), and so is its divisor.
+  const float up = top < 0x1p-100f ? 0x1p96f : 1.f, down = top < 0x1p-100f ? 0x1p-96f : 1.f;
+  const float d = __fdiv_rn(top * up, q_max(qt));
   // (rsqrt(..) of a finite sum is above 1e-20: a divisor of 1e-18 needs no look at the scale)
-  if (!writer && d >= 1e-18f) return d;
+  if (!writer && up == 1.f && d >= 1e-18f) return {d, up};
   // a sum of squares past the range of fp32 has no norm: NaN, not a scale of zero
   const float rstd = sum_sq < __uint_as_float(0x7f800000u)
                          ? __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps))
                          : __uint_as_float(0x7fc00000u);
-  const float s = rstd * d;
+  const float s = rstd * d * down;
   // a scale below 2^-126 is raised to it, and g's divisor with it (not to zero: g is zero or a few
   // of fp32's smallest steps there); NaN fails the test and stays
   const bool tiny = s < kTinyScale;
   if (writer) *scale = tiny ? kTinyScale : s;
-  return tiny ? fmaxf(__fdiv_rn(kTinyScale, rstd), __uint_as_float(1u)) : d;
+  return {tiny ? fmaxf(__fdiv_rn(kTinyScale * up, rstd), __uint_as_float(1u)) : d, up};
 }
 
 // Every kernel here is a programmatic dependent launch: it may be scheduled while the kernel before it
@@ -156,14 +166,14 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       sum += s_sum[i];
       mx = max(mx, s_max[i]);
     }
-    const float divisor = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
-    const bool finite = divisor <= 3.402823466e38f;
+    const Divisor by = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
+    const bool finite = by.d <= 3.402823466e38f;
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
     // sum_out may be x or the residual: an element is written by the thread that has just read it
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
       const float v = value(c, &h);
-      q[c] = finite ? encode8(__fdiv_rn(v, divisor), p.q_type) : 0;
+      q[c] = finite ? encode8(__fdiv_rn(v * by.up, by.d), p.q_type) : 0;
       if (KIND == FRISK_QUANT_RMSNORM && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
@@ -360,16 +370,18 @@ __device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TI
 
 // g over the divisor, in place.
 template <int NV>
-__device__ __forceinline__ void divide(f2 (&g)[NV][4], float d) {
-  if (!(d >= 1e-30f && d <= 3.402823466e38f)) {
+__device__ __forceinline__ void divide(f2 (&g)[NV][4], Divisor by) {
+  float d = by.d;
+  if (by.up != 1.f || !(d >= 1e-30f && d <= 3.402823466e38f)) {
     // a small divisor: both up by the same power of two (exact), so that div_by stays in range; a
     // divisor of infinity or NaN: zeros, next to a scale that makes every product NaN
     const bool small = d < 1.f;
-    d = small ? d * 0x1p96f : 1.f;
+    const float up = by.up == 1.f ? 0x1p96f : by.up;
+    if (by.up == 1.f) d = small ? d * up : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[i][j] = small ? mul2(g[i][j], pack2(0x1p96f)) : 0;
+      for (int j = 0; j < 4; ++j) g[i][j] = small ? mul2(g[i][j], pack2(up)) : 0;
   }
   const f2 minus_d = pack2(-d), y = pack2(__frcp_rn(d));
 #pragma unroll
@@ -499,7 +511,7 @@ __global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
     float sum = lo2(sums) + hi2(sums);
     uint32_t mx = __float_as_uint(top);
     row_fold<KIND>(sum, mx, s_sum, s_max, t >> 5, lane, 0, 32);
-    const float d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
+    const Divisor d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
 #pragma unroll 2
     for (int i = t; i < groups; i += 1024) {

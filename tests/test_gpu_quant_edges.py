@@ -1,0 +1,36 @@
+"""GPU checks of the 8-bit row makers where their arithmetic is at its limits: rows of the smallest
+numbers, ties, sums that leave fp32, gates far out.  Every case runs through each kernel that a width
+and an alignment choose; inputs are fp32 unless the case needs another type.  Tolerances are those of
+test_gpu_quant.py (u = 2^-24) unless a test derives its own."""
+import numpy as np
+import pytest
+
+from frisk_b200 import runtime as R
+from frisk_b200 import workloads as W
+from oracle import ref
+from test_gpu_quant import IN_TYPES, Q_TYPES, check_q, ids
+
+pytestmark = pytest.mark.gpu
+
+# in registers; off the 16-byte grid; two passes over aligned rows; element by element
+WIDTHS = [64, 1024, 1001, 40000, 40001]
+STEP = 2.0 ** -149   # fp32's smallest number
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_norms_of_the_smallest_numbers(cols, q_type):
+    """Rows of a few thousand of fp32's smallest steps, whose 8-bit scale is still a regular number:
+    with eps = 1e-10 a norm multiplies them by 1e5.  Nothing is rounded on the way to max |g| (no
+    weight), so q and the scale keep the tolerances of ordinary rows."""
+    top = {W.I8: 10710, W.E4M3: 37800, W.E5M2: 4838300}[q_type]   # the scale is about 1.18e-38, 2^-126 = 1.175e-38
+    rng = np.random.default_rng(cols)
+    n = rng.integers(-top, top + 1, (4, cols))
+    n[:, cols // 2] = top
+    n[1, cols // 3] = -top
+    x = (n.astype(np.float64) * STEP).astype(np.float32)
+    v, _ = ref.ref_quant(x, W.F32, "rmsnorm", eps=1e-10)
+    assert (ref.quant_scale(v, q_type) > 2.0 ** -126).all()
+    q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", eps=1e-10)
+    check_q(q, s, v, "rmsnorm", q_type)
+    assert (W.decode(q, q_type)[:, cols // 2] == W.QUANT_MAX[q_type]).all()
