@@ -83,39 +83,51 @@ __device__ __forceinline__ void warp_fold(float& sum, uint32_t& mx) {
 
 __device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 
-// What a row's elements are divided by: q = round(v * up / d).
-struct Divisor {
-  float d, up;
+// What a row's elements are multiplied by: q = round(v * up * (hi + lo)).  hi + lo is Q / max |v| as the
+// sum of two fp32 numbers (to 2^-46), not the reciprocal of the stored scale, whose rounding would move
+// every quotient of a row a little: an element exactly half way between two 8-bit numbers (half of the
+// maximum is 63.5 in int8) has to stay there to be rounded to even.  hi = 0: q is zero.
+struct Factor {
+  float hi, lo, up;
 };
 
-// scale[r] and the divisor of g from the row's sum of h^2 and maximum of |g| (as bits).  Every thread
-// of the row needs the divisor; the scale, with its root, only the one that stores it (`writer`).
+// scale[r] and the factor of g from the row's sum of h^2 and maximum of |g| (as bits).  Every thread
+// of the row needs the factor; the scale, with its root, only the one that stores it (`writer`).
 template <int KIND>
-__device__ __forceinline__ Divisor row_divisor(float sum_sq, uint32_t max_bits, int64_t cols, float eps, int qt,
-                                               bool writer, float* scale) {
-  const float top = __uint_as_float(max_bits);
+__device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, int64_t cols, float eps, int qt,
+                                             bool writer, float* scale) {
+  const float top = __uint_as_float(max_bits), q = q_max(qt);
+  // A norm's row of very small g: Q over its maximum would leave fp32, so the row is worked on 2^96 times
+  // as large (exact).
+  const bool low = KIND == FRISK_QUANT_RMSNORM && top < 0x1p-100f;
+  const float up = low ? 0x1p96f : 1.f, m = top * up;
+  Factor f{__fdiv_rn(q, m), 0.f, up};
+  f.lo = fmaf(-f.hi, m, q) * (qt == FRISK_DT_I8 ? 1.f / 127.f : qt == FRISK_DT_E4M3 ? 1.f / 448.f : 1.f / 57344.f) * f.hi;
+  if (max_bits >= 0x7f800000u) f = {0.f, 0.f, 1.f};   // zeros, next to a scale that makes every product NaN
   if (KIND != FRISK_QUANT_RMSNORM) {
-    const float d = __fdiv_rn(top, q_max(qt));
-    const float s = max_bits > 0x7f800000u ? d : fmaxf(d, kTinyScale);
-    if (writer) *scale = s;
-    return {s, 1.f};
+    const bool tiny = top < q * kTinyScale;   // the scale is 2^-126, and the factor 2^126
+    if (writer) *scale = tiny ? kTinyScale : __fdiv_rn(top, q);
+    if (tiny) f = {0x1p126f, 0.f, 1.f};
+    return f;
   }
-  // A row of very small g: its maximum over Q would be a subnormal number of a few bits, so the row is
-  // worked on 2^96 times as large (exact), and so is its divisor.
-  const float up = top < 0x1p-100f ? 0x1p96f : 1.f, down = top < 0x1p-100f ? 0x1p-96f : 1.f;
-  const float d = __fdiv_rn(top * up, q_max(qt));
-  // (rsqrt(..) of a finite sum is above 1e-20: a divisor of 1e-18 needs no look at the scale)
-  if (!writer && up == 1.f && d >= 1e-18f) return {d, up};
+  // (rsqrt(..) of a finite sum is above 1e-20: a maximum of 1e-12 needs no look at the scale)
+  if (!writer && top >= 1e-12f) return f;
   // a sum of squares past the range of fp32 has no norm: NaN, not a scale of zero
   const float rstd = sum_sq < __uint_as_float(0x7f800000u)
                          ? __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps))
                          : __uint_as_float(0x7fc00000u);
-  const float s = rstd * d * down;
-  // a scale below 2^-126 is raised to it, and g's divisor with it (not to zero: g is zero or a few
-  // of fp32's smallest steps there); NaN fails the test and stays
+  const float s = rstd * __fdiv_rn(m, q) * (low ? 0x1p-96f : 1.f);
+  // a scale below 2^-126 is raised to it, and the factor goes with it; NaN fails the test and stays
   const bool tiny = s < kTinyScale;
   if (writer) *scale = tiny ? kTinyScale : s;
-  return {tiny ? fmaxf(__fdiv_rn(kTinyScale * up, rstd), __uint_as_float(1u)) : d, up};
+  if (tiny) f = {rstd * (low ? 0x1p30f : 0x1p126f), 0.f, up};
+  return f;
+}
+// v * up * (hi + lo), to 2^-24 of it: exact where that is an fp32 number.
+__device__ __forceinline__ float times(float v, Factor f) {
+  if (f.hi == 0.f) return 0.f;
+  v *= f.up;
+  return fmaf(v, f.hi, v * f.lo);
 }
 
 // Every kernel here is a programmatic dependent launch: it may be scheduled while the kernel before it
@@ -166,14 +178,13 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       sum += s_sum[i];
       mx = max(mx, s_max[i]);
     }
-    const Divisor by = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
-    const bool finite = by.d <= 3.402823466e38f;
+    const Factor f = row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
     // sum_out may be x or the residual: an element is written by the thread that has just read it
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
       const float v = value(c, &h);
-      q[c] = finite ? encode8(__fdiv_rn(v * by.up, by.d), p.q_type) : 0;
+      q[c] = encode8(times(v, f), p.q_type);
       if (KIND == FRISK_QUANT_RMSNORM && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
@@ -309,7 +320,8 @@ __device__ __forceinline__ void encode_groups(const f2 (&v)[NV][4], int qt, uint
 // gate / (1 + exp(-gate)) * up for two elements.  e = exp(-gate) = 2^t, t = -gate log2(e): the product
 // is split into its rounded value, for the hardware's 2^x, and the exact rest, which with log2(e)'s own
 // rest enters to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's, corrected by
-// its remainder as in div_by.  The exponent is taken of gates held to [-88, 200]: above, e is zero
+// its remainder, which is exact in one fused multiply-add (P. Markstein, IBM Journal of Research and
+// Development 34(1), 1990).  The exponent is taken of gates held to [-88, 200]: above, e is zero
 // already; at -88 the reciprocal of 1 + e is below 2^-126, which the hardware flushes to zero, so
 // gates below -87.3 give zero (gate = NaN still enters as the dividend).
 __device__ __forceinline__ f2 silu_mul2(f2 gate, f2 up) {
@@ -325,15 +337,6 @@ __device__ __forceinline__ f2 silu_mul2(f2 gate, f2 up) {
   const f2 y = pack2(rcp(-lo2(minus_d)), rcp(-hi2(minus_d)));
   const f2 s = mul2(gate, y);
   return mul2(fma2(fma2(s, minus_d, gate), y, s), up);
-}
-
-// v / d to nearest for many v and one d: with y the reciprocal of d to nearest and q = v y, the
-// remainder v - q d is exact in one fused multiply-add, and q plus the remainder times y is the
-// correctly rounded quotient (P. Markstein, IBM Journal of Research and Development 34(1), 1990) where
-// nothing leaves the range of normal numbers: d is at least 1e-30 and finite here, and v at most Q d.
-__device__ __forceinline__ f2 div_by(f2 v, f2 minus_d, f2 y) {
-  const f2 q = mul2(v, y);
-  return fma2(fma2(q, minus_d, v), y, q);
 }
 
 // Eight elements from storage to g, with the running sum of squares and maximum.  `weights(v)` fills v
@@ -368,26 +371,20 @@ __device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TI
   for (int j = 0; j < 4; ++j) top = abs_max(g[j], top);
 }
 
-// g over the divisor, in place.
+// g times the row's factor, in place.
 template <int NV>
-__device__ __forceinline__ void divide(f2 (&g)[NV][4], Divisor by) {
-  float d = by.d;
-  if (by.up != 1.f || !(d >= 1e-30f && d <= 3.402823466e38f)) {
-    // a small divisor: both up by the same power of two (exact), so that div_by stays in range; a
-    // divisor of infinity or NaN: zeros, next to a scale that makes every product NaN
-    const bool small = d < 1.f;
-    const float up = by.up == 1.f ? 0x1p96f : by.up;
-    if (by.up == 1.f) d = small ? d * up : 1.f;
+__device__ __forceinline__ void multiply(f2 (&g)[NV][4], Factor f) {
+  if (f.up != 1.f || f.hi == 0.f) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g[i][j] = small ? mul2(g[i][j], pack2(up)) : 0;
+      for (int j = 0; j < 4; ++j) g[i][j] = f.hi == 0.f ? 0 : mul2(g[i][j], pack2(f.up));
   }
-  const f2 minus_d = pack2(-d), y = pack2(__frcp_rn(d));
+  const f2 hi = pack2(f.hi), lo = pack2(f.lo);
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[i][j] = div_by(g[i][j], minus_d, y);
+    for (int j = 0; j < 4; ++j) g[i][j] = fma2(g[i][j], hi, mul2(g[i][j], lo));
 }
 
 // Sum and maximum over the `wpr` warps of each of the CTA's rows, in every thread (a CTA barrier).
@@ -463,7 +460,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   uint32_t mx = __float_as_uint(top);
   row_fold<KIND>(sum, mx, s_sum, s_max, warp, lane, slot, wpr);
   if (!live) return;
-  divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
   uint2 bytes[NV];
   encode_groups<NV>(g, p.q_type, bytes);
@@ -511,12 +508,12 @@ __global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
     float sum = lo2(sums) + hi2(sums);
     uint32_t mx = __float_as_uint(top);
     row_fold<KIND>(sum, mx, s_sum, s_max, t >> 5, lane, 0, 32);
-    const Divisor d = row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
+    const Factor f = row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
 #pragma unroll 2
     for (int i = t; i < groups; i += 1024) {
       values(8 * (int64_t)i, true, sums, top);
-      divide<1>(g, d);
+      multiply<1>(g, f);
       uint2 bytes[1];
       encode_groups<1>(g, p.q_type, bytes);
       *reinterpret_cast<uint2*>(q + 8 * (int64_t)i) = bytes[0];
@@ -733,7 +730,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
   uint32_t mx = __float_as_uint(top);
   row_fold<KIND>(sum, mx, s_sum, s_max, slot * wpr + warp_in_row, lane, slot, wpr);
   if (!live) return;
-  divide<NV>(g, row_divisor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint2 bytes[NV];
   encode_groups<NV>(g, p.q_type, bytes);
   uint32_t qw[NV][2];
@@ -752,7 +749,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
 // 8192 as it is 50 against 55).
 // One CTA per SM walks the rows blockIdx.x, + gridDim.x, ...; bulk copies bring them into a ring of
 // `stages` whole rows (both operands), several ahead of the arithmetic, so that the memory is read
-// without a pause while rows are folded, divided and stored.  The CTA is blockDim.y teams of
+// without a pause while rows are folded, scaled and stored.  The CTA is blockDim.y teams of
 // blockDim.x threads; a team takes every blockDim.y-th row, so that one team's barrier is another's
 // arithmetic.  The row's stage is refilled as soon as its team has read it into registers.
 // Waits are bounded: a team whose copies do not arrive gives up and leaves NaN in its rows' scales.
@@ -880,7 +877,7 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
     if (t == 0 && j + stages < n) fetch(j + stages, stage);
     mx = lane < wpr ? s_max[buf][team * wpr + lane] : 0u;
     warp_fold<FRISK_QUANT_SILU_MUL>(sum, mx);
-    divide<NV>(g, row_divisor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+    multiply<NV>(g, row_factor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     uint2 eight[NV];
     encode_groups<NV>(g, p.q_type, eight);

@@ -34,3 +34,26 @@ def test_norms_of_the_smallest_numbers(cols, q_type):
     q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", eps=1e-10)
     check_q(q, s, v, "rmsnorm", q_type)
     assert (W.decode(q, q_type)[:, cols // 2] == W.QUANT_MAX[q_type]).all()
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("in_type", [W.F16, W.BF16], ids=ids)
+@pytest.mark.parametrize("rows,cols", [(64, 64), (700, 1024), (700, 1001), (40, 3001), (3, 40000), (3, 40001)])
+def test_ties_of_16_bit_rows_fall_as_defined(rows, cols, in_type, q_type):
+    """q is the rounding of v Q / max |v|, ties to even, for 16-bit rows WITHOUT any allowance: with v = a 2^i
+    and max = b 2^j, a and b whole numbers below 2^11, and Q = 127, 7 * 2^6 or 7 * 2^13, the quotient and a
+    border between two 8-bit numbers, an odd number below 2^8 times a power of two, differ by a whole number
+    over 255 * 2047 of the larger at least, if they differ: 2^-19, and the quotient is good to 2^-23.  The
+    values are multiples of a few steps, so that many quotients are borders."""
+    rng = np.random.default_rng([7, rows, cols, in_type])
+    x = (rng.integers(-64, 65, (rows, cols)) * 2.0 ** rng.integers(-6, 7, (rows, 1))).astype(np.float32)
+    x[rows // 2:] = (rng.standard_normal((rows - rows // 2, cols)) * 3).astype(np.float32)
+    x = W.encode(x, in_type)
+    v, _ = ref.ref_quant(x, in_type, "plain")
+    want = ref.quant_scale(v, q_type)
+    q, s = R.quant_host(x, in_type, q_type)
+    got = W.decode(q, q_type).astype(np.float64)
+    t = v * W.QUANT_MAX[q_type] / np.abs(v).max(axis=1)[:, None]   # one rounding of a short product's quotient
+    bad = got != ref.round8(t, q_type)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.size} values, first at {tuple(np.argwhere(bad)[0])}"
+    assert (np.abs(s - want) <= 2.0 ** -24 * want).all()
