@@ -103,7 +103,10 @@ __device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, in
   const float up = low ? 0x1p96f : 1.f, m = top * up;
   Factor f{__fdiv_rn(q, m), 0.f, up};
   f.lo = fmaf(-f.hi, m, q) * (qt == FRISK_DT_I8 ? 1.f / 127.f : qt == FRISK_DT_E4M3 ? 1.f / 448.f : 1.f / 57344.f) * f.hi;
-  if (max_bits >= 0x7f800000u) f = {0.f, 0.f, 1.f};   // zeros, next to a scale that makes every product NaN
+  // zeros next to a scale that makes every product NaN; a sum of squares past the range of fp32 has no norm
+  // and gets one as well
+  const bool no_norm = KIND == FRISK_QUANT_RMSNORM && !(sum_sq < __uint_as_float(0x7f800000u));
+  if (max_bits >= 0x7f800000u || no_norm) f = {0.f, 0.f, 1.f};
   if (KIND != FRISK_QUANT_RMSNORM) {
     const bool tiny = top < q * kTinyScale;   // the scale is 2^-126, and the factor 2^126
     if (writer) *scale = tiny ? kTinyScale : __fdiv_rn(top, q);
@@ -112,10 +115,7 @@ __device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, in
   }
   // (rsqrt(..) of a finite sum is above 1e-20: a maximum of 1e-12 needs no look at the scale)
   if (!writer && top >= 1e-12f) return f;
-  // a sum of squares past the range of fp32 has no norm: NaN, not a scale of zero
-  const float rstd = sum_sq < __uint_as_float(0x7f800000u)
-                         ? __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps))
-                         : __uint_as_float(0x7fc00000u);
+  const float rstd = no_norm ? __uint_as_float(0x7fc00000u) : __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps));
   const float s = rstd * __fdiv_rn(m, q) * (low ? 0x1p-96f : 1.f);
   // a scale below 2^-126 is raised to it, and the factor goes with it; NaN fails the test and stays
   const bool tiny = s < kTinyScale;

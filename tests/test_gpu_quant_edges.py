@@ -57,3 +57,18 @@ def test_ties_of_16_bit_rows_fall_as_defined(rows, cols, in_type, q_type):
     bad = got != ref.round8(t, q_type)
     assert not bad.any(), f"{int(bad.sum())} of {bad.size} values, first at {tuple(np.argwhere(bad)[0])}"
     assert (np.abs(s - want) <= 2.0 ** -24 * want).all()
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("cols", [512] + WIDTHS)
+def test_rows_whose_squares_overflow_have_zeros_beside_their_scale(cols, q_type):
+    """A norm past fp32: NaN for the scale, zeros for q (also where the weight takes the row to zero)."""
+    x = np.random.default_rng(cols).uniform(1, 2, (4, cols)).astype(np.float32)
+    x[0] *= 1e25
+    x[1, cols - 1] = 3e38
+    x[2, 0] = -1e20
+    w = np.ones(cols, np.float32)
+    for weight in (None, w, 0 * w):
+        q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", weight=weight)
+        assert np.isnan(s[:3]).all() and not q[:3].any()
+        assert np.isfinite(s[3]) and bool(q[3].any()) == (weight is None or bool(weight.any()))
