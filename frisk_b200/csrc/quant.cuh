@@ -115,7 +115,10 @@ __device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, in
   }
   // (rsqrt(..) of a finite sum is above 1e-20: a maximum of 1e-12 needs no look at the scale)
   if (!writer && top >= 1e-12f) return f;
-  const float rstd = no_norm ? __uint_as_float(0x7fc00000u) : __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(sum_sq, (float)cols) + eps));
+  const float mean = __fdiv_rn(sum_sq, (float)cols);
+  float rstd = __fdiv_rn(1.f, __fsqrt_rn(mean + eps));
+  if (rstd == 0.f) rstd = __fdiv_rn(0.5f, __fsqrt_rn(0.25f * mean + 0.25f * eps));   // the sum alone left fp32
+  if (no_norm) rstd = __uint_as_float(0x7fc00000u);
   const float s = rstd * __fdiv_rn(m, q) * (low ? 0x1p-96f : 1.f);
   // a scale below 2^-126 is raised to it, and the factor goes with it; NaN fails the test and stays
   const bool tiny = s < kTinyScale;

@@ -72,3 +72,15 @@ def test_rows_whose_squares_overflow_have_zeros_beside_their_scale(cols, q_type)
         q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", weight=weight)
         assert np.isnan(s[:3]).all() and not q[:3].any()
         assert np.isfinite(s[3]) and bool(q[3].any()) == (weight is None or bool(weight.any()))
+
+
+@pytest.mark.parametrize("cols", [1, 17, 64, 1000])
+def test_eps_as_large_as_fp32_allows(cols):
+    """mean + eps may leave fp32's range although neither does: the factor 1 / rms is that of the sum."""
+    eps = 3.4e38
+    x = np.random.default_rng(cols).uniform(0.5, 1, (3, cols)).astype(np.float32)
+    x *= np.float32(1.8e19 / np.sqrt(cols))
+    v, _ = ref.ref_quant(x, W.F32, "rmsnorm", eps=eps)
+    for q_type in Q_TYPES:
+        q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", eps=eps)
+        check_q(q, s, v, "rmsnorm", q_type)
