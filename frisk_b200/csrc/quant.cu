@@ -95,6 +95,10 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   if (p.cols > 8 * 1024 * kMaxGroups || p.rows > kMaxCtas) {   // ... or rows than a grid has CTAs
     return go(frisk_quant::quant_rows_generic_kernel<TIn, TW, KIND>, std::min(p.rows, kMaxCtas), dim3(256), 0, p, st);
   }
+  // Rows that may have to be looked at again (small_norm_row): a CTA each, and a sum in place of x or of
+  // the residual waits for that.
+  constexpr bool small_norms = KIND == frisk_quant::kNormAnyEps;
+  p.late_sum = small_norms && p.sum_out && (p.sum_out == p.x || p.sum_out == p.other);
   const int64_t groups = ceil_div(p.cols, 8);
   if constexpr (KIND == FRISK_QUANT_SILU_MUL) {
     // Streamed from two fillings of all SMs' rings on (bf16 / f16, in registers -> streamed: 67 MB of
@@ -122,7 +126,7 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   int nv = few ? 1 : aligned || (es == 2 && KIND == FRISK_QUANT_PLAIN) ? kMaxGroups : 2;
   while (ceil_div(groups, 32 * nv) > 32) nv *= 2;
   while (nv > 1 && 32 * (nv / 2) >= groups) nv /= 2;   // short rows: no more than a warp can use
-  const int wpr = (int)ceil_div(groups, 32 * nv), rows_per_cta = std::max(1, 8 / wpr);
+  const int wpr = (int)ceil_div(groups, 32 * nv), rows_per_cta = small_norms ? 1 : std::max(1, 8 / wpr);
   const int64_t ctas = ceil_div(p.rows, rows_per_cta);
   const dim3 threads(32 * wpr, rows_per_cta);
   const bool full = p.cols == 256ll * nv * wpr && p.rows % rows_per_cta == 0;
@@ -132,7 +136,7 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
     kern = nv == 1   ? quant_rows_unaligned_kernel<TIn, TW, KIND, 1>
            : nv == 2 ? quant_rows_unaligned_kernel<TIn, TW, KIND, 2>
                      : quant_rows_unaligned_kernel<TIn, TW, KIND, 4>;
-  else if (full)
+  else if (full && !small_norms)
     kern = nv == 1   ? quant_rows_kernel<TIn, TW, KIND, 1, true>
            : nv == 2 ? quant_rows_kernel<TIn, TW, KIND, 2, true>
                      : quant_rows_kernel<TIn, TW, KIND, 4, true>;
@@ -148,10 +152,14 @@ cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, int device, 
   switch (d.kind) {
     case FRISK_QUANT_PLAIN: return launch<TIn, TIn, FRISK_QUANT_PLAIN>(p, device, sms, st);
     case FRISK_QUANT_SILU_MUL: return launch<TIn, TIn, FRISK_QUANT_SILU_MUL>(p, device, sms, st);
-    default:
-      return d.weight_type == d.in_type ? launch<TIn, TIn, FRISK_QUANT_RMSNORM>(p, device, sms, st)
-                                        : launch<TIn, float, FRISK_QUANT_RMSNORM>(p, device, sms, st);
+    default: break;
   }
+  if (d.eps < frisk_quant::kSmallNorm) {
+    return d.weight_type == d.in_type ? launch<TIn, TIn, frisk_quant::kNormAnyEps>(p, device, sms, st)
+                                      : launch<TIn, float, frisk_quant::kNormAnyEps>(p, device, sms, st);
+  }
+  return d.weight_type == d.in_type ? launch<TIn, TIn, FRISK_QUANT_RMSNORM>(p, device, sms, st)
+                                    : launch<TIn, float, FRISK_QUANT_RMSNORM>(p, device, sms, st);
 }
 
 }  // namespace

@@ -26,6 +26,17 @@
 namespace frisk_quant {
 
 constexpr float kTinyScale = 1.17549435e-38f;   // 2^-126: 1 / scale is finite, q of a zero row is 0
+// A norm with mean(h^2) + eps below this, 1 / rms above 2^20: fp32 loses the squares of small h, and g =
+// h * weight may be a few of its smallest steps although the row's scale is a regular number.  Such rows,
+// possible only with an eps below it, are worked out in 64 bits (small_norm_row).  Above it a square that
+// is lost changes the mean by less than 2^-109 of it, and a row whose scale is regular has a maximum of 2^10
+// steps or more.
+constexpr float kSmallNorm = 0x1p-40f;
+// The kinds as template arguments: frisk_quant_kind, and the norm with an eps below kSmallNorm (in the
+// ordinary norm's kernels the mere presence of small_norm_row cost 8 % of 8192 x 8192 bf16, 30 % of
+// 1023 x 5001 f16).
+constexpr int kNormAnyEps = FRISK_QUANT_SILU_MUL + 1;
+constexpr bool is_norm(int kind) { return kind == FRISK_QUANT_RMSNORM || kind == kNormAnyEps; }
 
 struct Params {
   const void* x;
@@ -39,6 +50,7 @@ struct Params {
   float eps;
   int32_t q_type;
   int32_t stages;       // streamed rows: rows in the ring
+  int32_t late_sum;     // rmsnorm, rows in registers: sum_out is written when nothing of the row is needed any more
 };
 
 template <typename T>
@@ -74,7 +86,7 @@ __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v
 // Sum and maximum over a warp, in every lane.
 template <int KIND>
 __device__ __forceinline__ void warp_fold(float& sum, uint32_t& mx) {
-  if (KIND == FRISK_QUANT_RMSNORM) {
+  if (is_norm(KIND)) {
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   }
@@ -99,15 +111,15 @@ __device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, in
   const float top = __uint_as_float(max_bits), q = q_max(qt);
   // A norm's row of very small g: Q over its maximum would leave fp32, so the row is worked on 2^96 times
   // as large (exact).
-  const bool low = KIND == FRISK_QUANT_RMSNORM && top < 0x1p-100f;
+  const bool low = is_norm(KIND) && top < 0x1p-100f;
   const float up = low ? 0x1p96f : 1.f, m = top * up;
   Factor f{__fdiv_rn(q, m), 0.f, up};
   f.lo = fmaf(-f.hi, m, q) * (qt == FRISK_DT_I8 ? 1.f / 127.f : qt == FRISK_DT_E4M3 ? 1.f / 448.f : 1.f / 57344.f) * f.hi;
   // zeros next to a scale that makes every product NaN; a sum of squares past the range of fp32 has no norm
   // and gets one as well
-  const bool no_norm = KIND == FRISK_QUANT_RMSNORM && !(sum_sq < __uint_as_float(0x7f800000u));
+  const bool no_norm = is_norm(KIND) && !(sum_sq < __uint_as_float(0x7f800000u));
   if (max_bits >= 0x7f800000u || no_norm) f = {0.f, 0.f, 1.f};
-  if (KIND != FRISK_QUANT_RMSNORM) {
+  if (!is_norm(KIND)) {
     const bool tiny = top < q * kTinyScale;   // the scale is 2^-126, and the factor 2^126
     if (writer) *scale = tiny ? kTinyScale : __fdiv_rn(top, q);
     if (tiny) f = {0x1p126f, 0.f, 1.f};
@@ -141,6 +153,61 @@ __device__ __forceinline__ void after_the_kernel_before() {
   frisk::ptx::griddep_wait();
 }
 
+// Whether a row's norm is one for small_norm_row (the same in every thread of the row).
+__device__ __forceinline__ bool small_norm(float sum_sq, uint32_t max_bits, const Params& p) {
+  return p.eps < kSmallNorm && max_bits < 0x7f800000u && __fdiv_rn(sum_sq, (float)p.cols) + p.eps < kSmallNorm;
+}
+
+// One row after a norm in 64 bits, by a CTA: h in fp32 like everywhere, its squares, their sum
+// and h * weight in double (no range is left, the product is exact), q rounded from fp32.  Two passes over
+// the row, element by element; the sum is stored in the second, by the thread that has read the element.
+template <typename TIn, typename TW>
+__device__ __noinline__ void small_norm_row(const Params& p, int64_t r) {
+  __shared__ double s_sum[32], s_top[32];
+  const TIn* x = static_cast<const TIn*>(p.x) + r * p.ldx;
+  const TIn* o = p.other ? static_cast<const TIn*>(p.other) + r * p.ldo : nullptr;
+  const TW* w = static_cast<const TW*>(p.weight);
+  TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
+  auto value = [&](int64_t c, float* h) {
+    *h = to_float<TIn>(x[c]);
+    if (o) *h += to_float<TIn>(o[c]);
+    return w ? (double)*h * (double)to_float<TW>(w[c]) : (double)*h;
+  };
+  double sum = 0., top = 0.;
+  float h;
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    top = fmax(top, fabs(value(c, &h)));
+    sum += (double)h * h;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+  }
+  __syncthreads();   // a row before this one may still be reading the shared arrays
+  if ((threadIdx.x & 31) == 0) {
+    s_sum[threadIdx.x >> 5] = sum;
+    s_top[threadIdx.x >> 5] = top;
+  }
+  __syncthreads();
+  sum = top = 0.;
+  for (int i = 0; i < (int)blockDim.x / 32; ++i) {
+    sum += s_sum[i];
+    top = fmax(top, s_top[i]);
+  }
+  // (a row of zeros, which has no norm without eps: q = 0 and the least scale)
+  const double rstd = top == 0. ? 0. : 1. / sqrt(sum / (double)p.cols + (double)p.eps);
+  const double scale = top * rstd / q_max(p.q_type);
+  const bool tiny = scale < kTinyScale;
+  const double f = tiny ? rstd * 0x1p126 : q_max(p.q_type) / top;
+  if (threadIdx.x == 0) p.scale[r] = tiny ? kTinyScale : (float)scale;
+  uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
+  for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
+    q[c] = encode8((float)(value(c, &h) * f), p.q_type);
+    if (so) so[c] = from_float<TIn>(h);
+  }
+}
+
 // The plain form of the three kinds: a CTA per row, two passes over it, element by element.  Serves
 // any type, pitch, alignment and width.
 template <typename TIn, typename TW, int KIND>
@@ -156,7 +223,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
     auto value = [&](int64_t c, float* h) {
       float v = to_float<TIn>(x[c]);
       if (KIND == FRISK_QUANT_SILU_MUL) return silu_mul(v, to_float<TIn>(o[c]));
-      if (KIND == FRISK_QUANT_RMSNORM) {
+      if (is_norm(KIND)) {
         if (o) v += to_float<TIn>(o[c]);
         *h = v;
         if (w) v *= to_float<TW>(w[c]);
@@ -167,7 +234,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
     uint32_t mx = 0;
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
       mx = max(mx, abs_bits(value(c, &h)));
-      if (KIND == FRISK_QUANT_RMSNORM) sum = fmaf(h, h, sum);
+      if (is_norm(KIND)) sum = fmaf(h, h, sum);
     }
     warp_fold<KIND>(sum, mx);
     if ((threadIdx.x & 31) == 0) {
@@ -181,6 +248,13 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
       sum += s_sum[i];
       mx = max(mx, s_max[i]);
     }
+    if constexpr (KIND == kNormAnyEps) {
+      if (small_norm(sum, mx, p)) {
+        small_norm_row<TIn, TW>(p, r);
+        __syncthreads();
+        continue;
+      }
+    }
     const Factor f = row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, threadIdx.x == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     TIn* so = p.sum_out ? static_cast<TIn*>(p.sum_out) + r * p.lds : nullptr;
@@ -188,7 +262,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
       const float v = value(c, &h);
       q[c] = encode8(times(v, f), p.q_type);
-      if (KIND == FRISK_QUANT_RMSNORM && so) so[c] = from_float<TIn>(h);
+      if (is_norm(KIND) && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
   }
@@ -355,7 +429,7 @@ __device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TI
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = silu_mul2(g[j], u[j]);
   }
-  if (KIND == FRISK_QUANT_RMSNORM) {
+  if (is_norm(KIND)) {
     if (has_other) {
       unpack8(other, u);
 #pragma unroll
@@ -455,7 +529,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
             return w != nullptr;
           },
           [&](const f2 (&h)[4]) {
-            if (so) store8(so + 8 * (int64_t)gidx, h);
+            if (so && !(KIND == kNormAnyEps && p.late_sum)) store8(so + 8 * (int64_t)gidx, h);
           },
           g[i], sums, top);
   }
@@ -463,6 +537,9 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   uint32_t mx = __float_as_uint(top);
   row_fold<KIND>(sum, mx, s_sum, s_max, warp, lane, slot, wpr);
   if (!live) return;
+  if constexpr (KIND == kNormAnyEps) {
+    if (small_norm(sum, mx, p)) return small_norm_row<TIn, TW>(p, r);   // (the CTA has one row)
+  }
   multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
   uint2 bytes[NV];
@@ -471,6 +548,17 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   for (int i = 0; i < NV; ++i) {
     const int gidx = t + i * step;
     if (kFull || gidx < groups) *reinterpret_cast<uint2*>(q + 8 * (int64_t)gidx) = bytes[i];
+  }
+  if (KIND == kNormAnyEps && p.late_sum) {
+#pragma unroll 1
+    for (int gidx = t; gidx < groups; gidx += step) {
+      f2 h[4], u[4];
+      unpack8(load8(x + 8 * (int64_t)gidx), h);
+      unpack8(load8(o + 8 * (int64_t)gidx), u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = add2(h[j], u[j]);
+      store8(so + 8 * (int64_t)gidx, h);
+    }
   }
 }
 
@@ -511,6 +599,13 @@ __global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
     float sum = lo2(sums) + hi2(sums);
     uint32_t mx = __float_as_uint(top);
     row_fold<KIND>(sum, mx, s_sum, s_max, t >> 5, lane, 0, 32);
+    if constexpr (KIND == kNormAnyEps) {
+      if (small_norm(sum, mx, p)) {
+        small_norm_row<TIn, TW>(p, r);
+        __syncthreads();
+        continue;
+      }
+    }
     const Factor f = row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r);
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
 #pragma unroll 2
@@ -723,15 +818,23 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
         },
         g[i], sums, top);
   }
+  auto store_sum = [&] {
+    if (p.sum_out)
+      store_ragged<sizeof(TIn), NV>(reinterpret_cast<unsigned char*>(static_cast<TIn*>(p.sum_out) + r * p.lds), c0, cols, hw, lane);
+  };
   if (KIND == FRISK_QUANT_RMSNORM && p.sum_out) {
     // h may take the place of x or of the residual, and what this warp stores lies in words that the
     // row's other warps read: they have to have read them
     __syncthreads();
-    store_ragged<sizeof(TIn), NV>(reinterpret_cast<unsigned char*>(static_cast<TIn*>(p.sum_out) + r * p.lds), c0, cols, hw, lane);
+    store_sum();
   }
   float sum = lo2(sums) + hi2(sums);
   uint32_t mx = __float_as_uint(top);
   row_fold<KIND>(sum, mx, s_sum, s_max, slot * wpr + warp_in_row, lane, slot, wpr);
+  if constexpr (KIND == kNormAnyEps) {
+    if (small_norm(sum, mx, p)) return small_norm_row<TIn, TW>(p, r);   // (the CTA has one row)
+    store_sum();   // (the row's reads are behind the fold)
+  }
   if (!live) return;
   multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint2 bytes[NV];

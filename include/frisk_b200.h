@@ -365,8 +365,10 @@ int frisk_b200_reduce_run_host(const frisk_reduce_desc* desc, const void* src, v
  *   scale[r] = max(max |v[r, :]| / Q, 2^-126),  q[r, c] = nearest-even(v[r, c] / scale[r])
  * with Q = 127 (i8: -128 is not used), 448 (e4m3), 57344 (e5m2).  Arithmetic in fp32 (the norm is of
  * the unrounded h; squares are summed in fp32, so the rows' norms have to stay below 1e19), one
- * rounding into q and one into sum_out.  A row with an infinity or NaN in v, or with squares that
- * overflow, gets a scale of infinity or NaN and zeros for q: every product with its scale is NaN.  A row of zeros gets q = 0 and the scale 2^-126.  The order of the sum is
+ * rounding into q and one into sum_out; rows with mean(h^2) + eps below 2^-40 = 9.1e-13, whose squares
+ * fp32 would lose, in fp64.  A row with an infinity or NaN in v, or with squares that
+ * overflow, gets a scale of infinity or NaN and zeros for q: every product with its scale is NaN.
+ * A row of zeros gets q = 0 and the scale 2^-126, without eps too.  The order of the sum is
  * fixed by the shape, the types and the alignment.
  */
 typedef enum {

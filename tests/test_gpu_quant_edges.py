@@ -84,3 +84,73 @@ def test_eps_as_large_as_fp32_allows(cols):
     for q_type in Q_TYPES:
         q, s = R.quant_host(x, W.F32, q_type, "rmsnorm", eps=eps)
         check_q(q, s, v, "rmsnorm", q_type)
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-13, 1e-10])
+@pytest.mark.parametrize("cols", [1] + WIDTHS)
+def test_norms_of_rows_whose_squares_fp32_does_not_hold(cols, eps):
+    """eps down to zero with rows from 1e-44 to 1e15 times a normal one: the norm is that of the row,
+    and a row of zeros has q = 0 and the scale 2^-126."""
+    rng = np.random.default_rng([cols, 3])
+    tops = [0.0, 1e-44, 1e-39, 1e-30, 1e-24, 1e-22, 1e-19, 1e-14, 1e-8, 1e-6, 1e-5, 1e-3, 1.0, 1e6, 1e15]
+    x = (rng.standard_normal((len(tops), cols)) * np.array(tops)[:, None]).astype(np.float32)
+    x[:, 0] = np.where(x[:, 0] == 0, np.array(tops, np.float32), x[:, 0])
+    r = (rng.standard_normal(x.shape) * np.array(tops)[:, None]).astype(np.float32)
+    w = (1 + 0.2 * rng.standard_normal(cols)).astype(np.float32)
+    for q_type in (W.I8, W.E4M3):
+        v, h = ref.ref_quant(x, W.F32, "rmsnorm", eps=eps, residual=r, weight=w)
+        q, s, total = R.quant_host(x, W.F32, q_type, "rmsnorm", eps=eps, residual=r, weight=w, want_sum=True)
+        h32 = x + r
+        assert np.array_equal(total, h32)
+        assert s[0] == np.float32(2.0 ** -126) and not W.decode(q[0], q_type).any()   # (-0 stays -0)
+        # h is rounded once; below 2^-126 by up to half a step of 2^-149, like h * weight where the rows'
+        # factor 1 / rms is at most 2^20 (beyond that the product is not rounded)
+        h64 = h32.astype(np.float64)
+        live = h64.any(axis=1)
+        rstd = np.where(live, 1 / np.sqrt(np.where(live, np.mean(h64 * h64, axis=1) + np.float64(np.float32(eps)), 1)), 0)
+        v = h64 * rstd[:, None] * w
+        want = ref.quant_scale(v, q_type)
+        terms = cols / 32 + 1 + 37
+        slack = np.where(rstd <= 2.0 ** 20, 2.0 ** -150 * rstd, 0.0)
+        err = np.abs(s.astype(np.float64) - want)
+        assert (err <= (terms / 2 + 9) * 2.0 ** -24 * want + slack / W.QUANT_MAX[q_type])[live].all(), (err / want)[live]
+        t = v / want[:, None]
+        a = np.abs(t) * 7 * 2.0 ** -24 + 2 * (slack / want)[:, None]
+        lo, hi = ref.round8(t - a, q_type), ref.round8(t + a, q_type)
+        clamped = want <= 2.0 ** -126 * (1 + 2.0 ** -20)   # the stored scale is the least one: v's own error shows
+        got = W.decode(q, q_type).astype(np.float64)
+        bad = ~((got >= lo) & (got <= hi)) & (live & ~clamped)[:, None]
+        assert not bad.any(), np.unique(np.argwhere(bad)[:, 0])
+        step = np.where(np.abs(t) < 1, 1, np.abs(t)) * (terms / 2 + 16) * 2.0 ** -24 + a
+        lo, hi = ref.round8(t - step, q_type), ref.round8(t + step, q_type)
+        assert (((got >= lo) & (got <= hi)) | ~(live & clamped)[:, None]).all()
+
+
+@pytest.mark.parametrize("in_type", IN_TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_eps_zero_with_the_sum_in_place(cols, in_type):
+    """Without eps, rows of ordinary and of very small numbers side by side; the sum over x or the residual."""
+    import torch
+    dev = torch.device("cuda:0")
+    rng = np.random.default_rng([cols, 4])
+    tops = np.array([1.0, 3e-7, 0.0, 2e-4, 6e-8, 40.0])[:, None]   # (6e-8: fp16's smallest numbers)
+    x, r = (W.encode((rng.standard_normal((6, cols)) * tops).astype(np.float32), in_type) for _ in range(2))
+    wt = W.encode((1 + 0.2 * rng.standard_normal(cols)).astype(np.float32), in_type)
+    v, h = ref.ref_quant(x, in_type, "rmsnorm", eps=0.0, residual=r, weight=wt)
+    on = lambda a: torch.from_numpy(np.ascontiguousarray(a).view(np.uint8)).to(dev)  # noqa: E731
+    desc, weight = R.quant_desc(6, cols, in_type, W.I8, "rmsnorm", eps=0.0), on(wt)
+    got = []
+    for where in ("apart", "x", "residual"):
+        bx, br = on(x), on(r)
+        total = torch.zeros_like(bx) if where == "apart" else bx if where == "x" else br
+        q, s = torch.zeros((6, cols), dtype=torch.int8, device=dev), torch.zeros(6, device=dev)
+        R.quant_run(desc, bx, q, s, weight=weight, residual=br, sum_out=total)
+        torch.cuda.synchronize()
+        got.append((q.cpu().numpy(), s.cpu().numpy(), total.cpu().numpy()))
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            assert np.array_equal(a, b)
+    q, s, _ = got[0]
+    live = h.any(axis=1)
+    check_q(q[live], s[live], v[live], "rmsnorm", W.I8)
+    assert not q[~live].any() and (s[~live] == np.float32(2.0 ** -126)).all()
