@@ -93,7 +93,33 @@ __device__ __forceinline__ void warp_fold(float& sum, uint32_t& mx) {
   mx = __reduce_max_sync(0xffffffffu, mx);
 }
 
-__device__ __forceinline__ float silu_mul(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// gate / (1 + exp(-gate)) * up.  Gates from -kNearGate on leave every step in fp32's normal numbers: exp(87)
+// is 6.1e37, and its reciprocal is above 2^-126.
+constexpr float kNearGate = 87.f;
+constexpr float kLog2e = 1.44269504f, kLog2eRest = (float)(1.4426950408889634074 - (double)1.44269504f), kLn2 = 0.693147181f;
+
+// Below, 1 + exp(-gate) is exp(-gate) in fp32, past its range from -88.7 on, though the product with a
+// large up is not: gate * (2^160 exp(gate)) * (2^-64 up) * 2^-96 rounds in the range of normal numbers until
+// the last step.  2^160 exp(gate) is zero from about -198 on, where the product with the largest up is
+// less than half of fp32's smallest number.
+__device__ __forceinline__ float silu_mul(float gate, float up) {
+  if (!(gate < -kNearGate)) return gate / (1.f + expf(-gate)) * up;
+  const float a = fmaxf(gate, -200.f), t = a * kLog2e;
+  const float rest = fmaf(a, kLog2eRest, fmaf(a, kLog2e, -t)) * kLn2;   // as in silu_mul2
+  const float e = ex2(t + 160.f);                                       // (the sum is exact)
+  return gate * fmaf(e, rest, e) * (up * 0x1p-64f) * 0x1p-96f;
+}
 
 // What a row's elements are multiplied by: q = round(v * up * (hi + lo)).  hi + lo is Q / max |v| as the
 // sum of two fp32 numbers (to 2^-46), not the reciprocal of the stored scale, whose rounding would move
@@ -324,14 +350,15 @@ __device__ __forceinline__ float abs_max(f2 v, float m) {
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(lo2(v)), "f"(hi2(v)), "f"(m));
   return r;
 }
-__device__ __forceinline__ float ex2(float v) {
+// min(a, b, m), NaN if one of them is, and max(a, b, m) of the numbers among them
+__device__ __forceinline__ float min3(f2 v, float m) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(lo2(v)), "f"(hi2(v)), "f"(m));
   return r;
 }
-__device__ __forceinline__ float rcp(float v) {
+__device__ __forceinline__ float max3(f2 v, float m) {
   float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(lo2(v)), "f"(hi2(v)), "f"(m));
   return r;
 }
 
@@ -394,26 +421,39 @@ __device__ __forceinline__ void encode_groups(const f2 (&v)[NV][4], int qt, uint
   else floats(__NV_E5M2);
 }
 
-// gate / (1 + exp(-gate)) * up for two elements.  e = exp(-gate) = 2^t, t = -gate log2(e): the product
-// is split into its rounded value, for the hardware's 2^x, and the exact rest, which with log2(e)'s own
-// rest enters to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's, corrected by
-// its remainder, which is exact in one fused multiply-add (P. Markstein, IBM Journal of Research and
-// Development 34(1), 1990).  The exponent is taken of gates held to [-88, 200]: above, e is zero
-// already; at -88 the reciprocal of 1 + e is below 2^-126, which the hardware flushes to zero, so
-// gates below -87.3 give zero (gate = NaN still enters as the dividend).
+// gate / (1 + exp(-gate)) * up for two gates from -kNearGate to kLargeGate.  e = exp(-gate) = 2^-t, t = gate
+// log2(e): the product is split into its rounded value, for the hardware's 2^x, and the exact rest, which
+// with log2(e)'s own rest enters to first order, 2^rest = 1 + rest ln 2.  The quotient is the reciprocal's,
+// corrected by its remainder, which is exact in one fused multiply-add (P. Markstein, IBM Journal of Research
+// and Development 34(1), 1990).
+constexpr float kLargeGate = 1e38f;   // t is finite
 __device__ __forceinline__ f2 silu_mul2(f2 gate, f2 up) {
-  constexpr float kLog2e = 1.44269504f, kLog2eRest = (float)(1.4426950408889634074 - (double)1.44269504f);
-  constexpr float kLn2 = 0.693147181f;
-  const f2 a = pack2(fminf(fmaxf(lo2(gate), -88.f), 200.f), fminf(fmaxf(hi2(gate), -88.f), 200.f));
-  const f2 t = mul2(a, pack2(kLog2e));
-  f2 rest = fma2(a, pack2(-kLog2e), t);
-  rest = mul2(fma2(a, pack2(-kLog2eRest), rest), pack2(kLn2));
+  const f2 t = mul2(gate, pack2(kLog2e));
+  f2 rest = fma2(gate, pack2(-kLog2e), t);
+  rest = mul2(fma2(gate, pack2(-kLog2eRest), rest), pack2(kLn2));
   f2 e = pack2(ex2(-lo2(t)), ex2(-hi2(t)));
   e = fma2(e, rest, e);
   const f2 minus_d = fma2(e, pack2(-1.f), pack2(-1.f));
   const f2 y = pack2(rcp(-lo2(minus_d)), rcp(-hi2(minus_d)));
   const f2 s = mul2(gate, y);
   return mul2(fma2(fma2(s, minus_d, gate), y, s), up);
+}
+// ... for any two: see silu_mul.
+__device__ __forceinline__ f2 silu_mul2_any(f2 gate, f2 up) {
+  const float g0 = lo2(gate), g1 = hi2(gate);
+  const bool far0 = g0 < -kNearGate, far1 = g1 < -kNearGate;
+  const f2 a = pack2(fminf(fmaxf(g0, -200.f), kNearGate), fminf(fmaxf(g1, -200.f), kNearGate));
+  const f2 t = mul2(a, pack2(kLog2e));
+  f2 rest = fma2(a, pack2(-kLog2e), t);
+  rest = mul2(fma2(a, pack2(-kLog2eRest), rest), pack2(kLn2));
+  f2 e = pack2(ex2(far0 ? lo2(t) + 160.f : -lo2(t)), ex2(far1 ? hi2(t) + 160.f : -hi2(t)));
+  e = fma2(e, pack2(far0 ? -lo2(rest) : lo2(rest), far1 ? -hi2(rest) : hi2(rest)), e);
+  const f2 minus_d = fma2(e, pack2(-1.f), pack2(-1.f));
+  const f2 y = pack2(rcp(-lo2(minus_d)), rcp(-hi2(minus_d)));
+  const f2 s = mul2(gate, y);
+  const f2 near = mul2(fma2(fma2(s, minus_d, gate), y, s), up), large = mul2(gate, up);
+  const f2 far = mul2(mul2(mul2(gate, e), mul2(up, pack2(0x1p-64f))), pack2(0x1p-96f));
+  return pack2(far0 ? lo2(far) : g0 > kNearGate ? lo2(large) : lo2(near), far1 ? hi2(far) : g1 > kNearGate ? hi2(large) : hi2(near));
 }
 
 // Eight elements from storage to g, with the running sum of squares and maximum.  `weights(v)` fills v
@@ -426,8 +466,19 @@ __device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TI
   f2 u[4];
   if (KIND == FRISK_QUANT_SILU_MUL) {
     unpack8(other, u);
+    float least = 0.f, most = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = silu_mul2(g[j], u[j]);
+    for (int j = 0; j < 4; ++j) {
+      least = min3(g[j], least);
+      most = max3(g[j], most);
+    }
+    if (least >= -kNearGate && most <= kLargeGate) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = silu_mul2(g[j], u[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = silu_mul2_any(g[j], u[j]);
+    }
   }
   if (is_norm(KIND)) {
     if (has_other) {

@@ -360,7 +360,8 @@ int frisk_b200_reduce_run_host(const frisk_reduce_desc* desc, const void* src, v
  *   FRISK_QUANT_RMSNORM   h = x + residual (no residual: h = x),
  *                         v = h * rsqrt(mean over the row of h^2 + eps) * weight (NULL: ones);
  *                         sum_out (may be NULL) = h rounded to the input type
- *   FRISK_QUANT_SILU_MUL  v = gate / (1 + exp(-gate)) * up, with x = gate and `up` the other matrix;
+ *   FRISK_QUANT_SILU_MUL  v = gate / (1 + exp(-gate)) * up, with x = gate and `up` the other matrix
+ *                         (also where exp(-gate) leaves fp32);
  *                         `up` NULL: x holds rows of 2 * cols elements, the gate and then the up half
  *   scale[r] = max(max |v[r, :]| / Q, 2^-126),  q[r, c] = nearest-even(v[r, c] / scale[r])
  * with Q = 127 (i8: -128 is not used), 448 (e4m3), 57344 (e5m2).  Arithmetic in fp32 (the norm is of

@@ -154,3 +154,58 @@ def test_eps_zero_with_the_sum_in_place(cols, in_type):
     live = h.any(axis=1)
     check_q(q[live], s[live], v[live], "rmsnorm", W.I8)
     assert not q[~live].any() and (s[~live] == np.float32(2.0 ** -126)).all()
+
+
+def far_gates(rows_of, cols, in_type, rng):
+    """Rows of gate and up with gates in bands from both ends: (values as stored, names)."""
+    bands = [(-88.7, -87.1), (-104.0, -88.8), (-140.0, -100.0), (-90.0, 90.0), (87.0, 300.0), (-190.0, -185.0)]
+    gate = np.stack([rng.uniform(*bands[i % len(bands)], cols) for i in range(rows_of)])
+    size = 1e4 if in_type == W.F16 else 1e35
+    up = rng.uniform(-size, size, (rows_of, cols))
+    return W.encode(np.concatenate([gate, up], axis=1).astype(np.float32), in_type), len(bands)
+
+
+def check_gates(q, s, x, in_type, q_type):
+    """As for ordinary gates (v carries 7 u); what leaves fp32's regular numbers on the way is rounded to
+    its smallest step once more, half a step of 2^-149."""
+    v, _ = ref.ref_quant(x, in_type, "silu_mul")
+    want = ref.quant_scale(v, q_type)
+    least = 2.0 ** -150
+    assert (np.abs(s - want) <= 9 * 2.0 ** -24 * want + least).all(), (s / want)
+    t = v / want[:, None]
+    a = np.abs(t) * 17 * 2.0 ** -24 + 2 * least / want[:, None]
+    lo, hi = ref.round8(t - a, q_type), ref.round8(t + a, q_type)
+    got = W.decode(q, q_type).astype(np.float64)
+    bad = ~((got >= lo) & (got <= hi))
+    assert not bad.any(), f"{int(bad.sum())} of {bad.size} values, first at {tuple(np.argwhere(bad)[0])}"
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("in_type", IN_TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_gates_far_from_zero(cols, in_type, q_type):
+    """exp(-gate) leaves fp32 below -88.7, and its reciprocal the regular numbers below -87.3; the product
+    with a large up does not."""
+    x, _ = far_gates(12, cols, in_type, np.random.default_rng([cols, 5]))
+    q, s = R.quant_host(x, in_type, q_type, "silu_mul")
+    check_gates(q, s, x, in_type, q_type)
+
+
+def test_gates_far_from_zero_in_streamed_rows():
+    x, _ = far_gates(4500, 4096, W.BF16, np.random.default_rng(6))
+    q, s = R.quant_host(x, W.BF16, W.E4M3, "silu_mul")
+    check_gates(q, s, x, W.BF16, W.E4M3)
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("cols", WIDTHS)
+def test_infinite_gates(cols, q_type):
+    """gate = infinity times up is an infinity, and so is the row's scale; -infinity * 0 is NaN."""
+    x = np.random.default_rng(cols).standard_normal((4, 2 * cols)).astype(np.float32)
+    x[0, cols // 2], x[0, cols + cols // 2] = np.inf, 2.0
+    x[1, 0] = -np.inf
+    x[2, cols - 1] = np.nan
+    q, s = R.quant_host(x, W.F32, q_type, "silu_mul")
+    assert np.isposinf(s[0]) and np.isnan(s[1:3]).all() and not q[:3].any()
+    v, _ = ref.ref_quant(x[3:], W.F32, "silu_mul")
+    check_q(q[3:], s[3:], v, "silu_mul", q_type)
