@@ -3,6 +3,7 @@
 #include "quant.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <string>
@@ -164,9 +165,17 @@ cudaError_t launch_kind(const frisk_quant_desc& d, const Params& p, int device, 
 
 }  // namespace
 
+std::atomic<int64_t> g_wait_cycles{frisk_quant::kRowWaitCycles};
+
 extern "C" {
 
+int64_t frisk_internal_quant_wait_cycles(int64_t cycles) { return g_wait_cycles.exchange(cycles); }
+
 int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* args) {
+  return frisk_b200_quant_run_status(desc, args, nullptr);
+}
+
+int frisk_b200_quant_run_status(const frisk_quant_desc* desc, const frisk_quant_args* args, int32_t* device_status) {
   if (!desc || !args) return FRISK_ERR_INVALID_ARGUMENT;
   const frisk_quant_desc& d = *desc;
   if (int rc = check_desc(d)) return rc;
@@ -185,6 +194,8 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
   p.ldq = d.ldq ? d.ldq : d.cols;
   p.eps = d.eps;
   p.q_type = d.q_type;
+  p.status = device_status;
+  p.wait_cycles = g_wait_cycles.load(std::memory_order_relaxed);
   if (d.rows == 0) return FRISK_OK;
   if (!args->x || !args->q || !args->scale) return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: null x, q or scale");
   const int es = in_bytes(d.in_type), ws = in_bytes(norm ? d.weight_type : d.in_type);
@@ -195,13 +206,13 @@ int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* a
   p.q = args->q;
   p.scale = args->scale;
   auto off = [](const void* ptr, int a) { return reinterpret_cast<uintptr_t>(ptr) % (unsigned)a != 0; };
-  if (off(p.x, es) || off(p.other, es) || off(p.weight, ws) || off(p.sum_out, es) || off(p.scale, 4))
+  if (off(p.x, es) || off(p.other, es) || off(p.weight, ws) || off(p.sum_out, es) || off(p.scale, 4) || off(p.status, 4))
     return fail(FRISK_ERR_MISALIGNED, "quant: a pointer is not aligned to its element size");
   // the sum may replace x or the residual, element for element
   if ((p.sum_out == p.x && p.sum_out && p.lds != p.ldx) || (p.sum_out == p.other && p.sum_out && p.lds != p.ldo))
     return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: sum_out in place of x or the residual needs the same pitch");
   // q and scale lie by themselves (the caller answers for partial overlaps)
-  for (const void* b : {p.x, p.other, p.weight, (const void*)p.sum_out})
+  for (const void* b : {p.x, p.other, p.weight, (const void*)p.sum_out, (const void*)p.status})
     if (b == p.q || b == p.scale || p.q == p.scale)
       return fail(FRISK_ERR_INVALID_ARGUMENT, "quant: q and scale must not be one of the other buffers");
   int prev = -1;
@@ -245,7 +256,8 @@ int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_ar
     int es;
   };
   const void* other = norm ? args->residual : gated ? args->up : nullptr;
-  enum { X, O, Wt, S, Q, Sc, N };
+  enum { X, O, Wt, S, Q, Sc, St, N };
+  int32_t status = 0;
   Buf b[N] = {
       {nullptr, args->x, nullptr, d.ldx ? d.ldx : xw, xw, d.rows, es},
       {nullptr, other, nullptr, d.ldo ? d.ldo : d.cols, d.cols, d.rows, es},
@@ -253,6 +265,7 @@ int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_ar
       {nullptr, nullptr, norm ? args->sum_out : nullptr, d.lds ? d.lds : d.cols, d.cols, d.rows, es},
       {nullptr, nullptr, args->q, d.ldq ? d.ldq : d.cols, d.cols, d.rows, 1},
       {nullptr, nullptr, args->scale, 1, 1, d.rows, 4},
+      {nullptr, &status, &status, 1, 1, 1, 4},
   };
   int prev = -1;
   cudaError_t e = cudaSuccess;
@@ -281,7 +294,7 @@ int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_ar
     a.stream = st;
     d.ldx = d.ldo = d.lds = d.ldq = 0;
     d.device = -1;
-    rc = frisk_b200_quant_run(&d, &a);
+    rc = frisk_b200_quant_run_status(&d, &a, static_cast<int32_t*>(b[St].dev));
     for (Buf& u : b)
       if (rc == FRISK_OK && e == cudaSuccess && u.out)
         e = cudaMemcpy2DAsync(u.out, u.ld * u.es, u.dev, u.width * u.es, u.width * u.es, u.rows, cudaMemcpyDeviceToHost, st);
@@ -291,6 +304,7 @@ int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_ar
     if (e == cudaSuccess) e = e2;
   }
   if (e != cudaSuccess && rc == FRISK_OK) rc = fail_cuda(e, "frisk_b200_quant_run_host");
+  if (status && rc == FRISK_OK) rc = fail(FRISK_ERR_DEVICE_TIMEOUT, "quant: a wait for rows ran out");
   for (Buf& u : b) cudaFree(u.dev);
   if (st) cudaStreamDestroy(st);
   if (prev >= 0 && prev != d.device) cudaSetDevice(prev);

@@ -50,6 +50,8 @@ struct Params {
   float eps;
   int32_t q_type;
   int32_t stages;       // streamed rows: rows in the ring
+  int32_t* status;      // streamed rows: where a wait that ran out is reported; nullptr: nowhere
+  int64_t wait_cycles;  // ... and how long a wait may take
   int32_t late_sum;     // rmsnorm, rows in registers: sum_out is written when nothing of the row is needed any more
 };
 
@@ -909,9 +911,12 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
 // without a pause while rows are folded, scaled and stored.  The CTA is blockDim.y teams of
 // blockDim.x threads; a team takes every blockDim.y-th row, so that one team's barrier is another's
 // arithmetic.  The row's stage is refilled as soon as its team has read it into registers.
-// Waits are bounded: a team whose copies do not arrive gives up and leaves NaN in its rows' scales.
+// Waits are bounded: a team whose copies do not arrive gives up, sets the status word and leaves NaN scales
+// and zeros for its rows from there on; the CTA stays until the copies that were asked for have landed.
 constexpr int kMaxRowStages = 16;
-constexpr long long kRowWaitCycles = 1ll << 29;   // about 0.3 s
+constexpr int64_t kRowWaitCycles = 1ll << 29;   // about 0.3 s
+constexpr int64_t kPollCycles = 1ll << 22;      // a poll counts as this at most
+constexpr int32_t kStatusRowsTimeout = 16;      // (the gemm kernels use the bits below)
 
 __device__ __forceinline__ uint32_t load_tag(uint32_t addr) {
   uint32_t v;
@@ -921,16 +926,26 @@ __device__ __forceinline__ uint32_t load_tag(uint32_t addr) {
 __device__ __forceinline__ void store_tag(uint32_t addr, uint32_t v) {
   asm volatile("st.release.cta.shared::cta.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
+// Polls a phase of the barrier `bar` until it is over and `also()` holds, for `limit` cycles: cycles of polling,
+// so that a CTA which did not run for a while (its context switched out) has not used its limit up, and with
+// a last look after them.
+template <typename Also>
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, int64_t limit, Also also) {
+  if (also() && frisk::ptx::mbar_test_wait(bar, parity)) return true;
+  for (long long last = clock64(); limit > 0;) {
+    if (also() && frisk::ptx::mbar_try_wait(bar, parity)) return true;
+    const long long now = clock64();
+    limit -= min((int64_t)(now - last), kPollCycles);
+    last = now;
+  }
+  return also() && frisk::ptx::mbar_test_wait(bar, parity);
+}
 // Waits for row `row` of this CTA in the stage behind `bar`.  A phase's parity alone does not say
 // which row it is: a team may be ahead of the one that has yet to read the stage's row before, and
 // would take the phase before that for its own.  So the stage's tag, set when a row is asked for,
 // comes first; from then on the barrier is in that row's phase or past it.
-__device__ __forceinline__ bool wait_row(uint32_t bar, uint32_t parity, uint32_t tag, uint32_t row) {
-  if (load_tag(tag) == row && frisk::ptx::mbar_try_wait(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (clock64() - t0 < kRowWaitCycles)
-    if (load_tag(tag) == row && frisk::ptx::mbar_try_wait(bar, parity)) return true;
-  return false;
+__device__ __forceinline__ bool wait_row(uint32_t bar, uint32_t parity, uint32_t tag, uint32_t row, int64_t limit) {
+  return poll(bar, parity, limit, [&] { return load_tag(tag) == row; });
 }
 // Barrier of one team (hardware barrier 1 + team): true if any thread brings `bad`.
 __device__ __forceinline__ bool team_barrier(int team, int threads, bool bad) {
@@ -964,7 +979,7 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ __align__(8) uint64_t bars[kMaxRowStages];
   __shared__ uint32_t tags[kMaxRowStages];   // which of the CTA's rows a stage was last asked for
-  __shared__ uint32_t s_max[2][32];
+  __shared__ uint32_t s_max[2][32], gave_up;
   const int t = threadIdx.x, step = blockDim.x, lane = t & 31, wpr = step >> 5;
   const int teams = blockDim.y, stages = p.stages;
   const int team = __shfl_sync(0xffffffffu, threadIdx.y, 0), warp = team * wpr + (t >> 5);
@@ -988,6 +1003,7 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
       frisk::ptx::mbar_init(bar0 + 8 * s, 1);
       tags[s] = 0xffffffffu;   // (n is below that: checked when launching)
     }
+    gave_up = 0;
     frisk::ptx::fence_mbar_init();
   }
   after_the_kernel_before();
@@ -1001,7 +1017,7 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
   int buf = 0;
   for (int64_t j = team; j < n; j += teams) {   // teams <= stages
     const int64_t r = blockIdx.x + j * gridDim.x;
-    const bool ok = wait_row(bar0 + 8 * stage, phase, tag0 + 4 * stage, (uint32_t)j);
+    const bool ok = wait_row(bar0 + 8 * stage, phase, tag0 + 4 * stage, (uint32_t)j, p.wait_cycles);
     const uint32_t at = ring0 + stage * stage_bytes;
     f2 g[NV][4];
     f2 sums = 0;
@@ -1023,10 +1039,14 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
     if (lane == 0) s_max[buf][warp] = mx;
     if (team_barrier(team, step, !ok)) {
       if (t == 0) {
-        const long long t0 = clock64();   // copies in flight land before the CTA may leave
-        while (clock64() - t0 < 100000ll) {
-        }
-        for (; j < n; j += teams) p.scale[blockIdx.x + j * gridDim.x] = __uint_as_float(0x7fc00000u);
+        gave_up = 1;
+        if (p.status) atomicOr(p.status, kStatusRowsTimeout);
+      }
+      for (; j < n; j += teams) {
+        const int64_t left = blockIdx.x + j * gridDim.x;
+        if (t == 0) p.scale[left] = __uint_as_float(0x7fc00000u);
+        for (int gidx = t; gidx < groups; gidx += step)
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + left * p.ldq + 8 * gidx) = make_uint2(0, 0);
       }
       break;
     }
@@ -1048,6 +1068,14 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
     if (stage >= stages) {
       stage -= stages;
       phase ^= 1u;
+    }
+  }
+  __syncthreads();   // no more rows are asked for
+  if (gave_up && threadIdx.x == 0 && threadIdx.y == 0) {   // the last row of every stage lands before the CTA leaves
+    for (int s = 0; s < stages; ++s) {
+      const uint32_t row = load_tag(tag0 + 4 * s);
+      if (row == 0xffffffffu) continue;
+      poll(bar0 + 8 * s, row / stages & 1u, kRowWaitCycles, [] { return true; });
     }
   }
 }

@@ -199,6 +199,8 @@ def lib() -> C.CDLL:
     L.frisk_b200_reduce_run_host.restype = C.c_int
     L.frisk_b200_quant_run.argtypes = [C.POINTER(QuantDesc), C.c_char_p]
     L.frisk_b200_quant_run.restype = C.c_int
+    L.frisk_b200_quant_run_status.argtypes = [C.POINTER(QuantDesc), C.c_char_p, vp]
+    L.frisk_b200_quant_run_status.restype = C.c_int
     L.frisk_b200_quant_run_host.argtypes = [C.POINTER(QuantDesc), C.c_char_p]
     L.frisk_b200_quant_run_host.restype = C.c_int
     L.frisk_b200_measure_mma_peak.argtypes = [C.c_int32, C.c_int32, C.c_int32, C.c_int32,
@@ -427,9 +429,12 @@ def _quant_args(x, q, scale, weight, residual, up, sum_out, stream) -> bytes:
 
 
 def quant_run(desc: QuantDesc, x, q, scale, *, weight=None, residual=None, up=None, sum_out=None,
-              stream: int = 0) -> None:
-    """Asynchronous launch on device buffers (torch CUDA tensors or raw addresses)."""
-    rc = (_lib or lib()).frisk_b200_quant_run(C.byref(desc), _quant_args(x, q, scale, weight, residual, up, sum_out, stream))
+              stream: int = 0, status=None) -> None:
+    """Asynchronous launch on device buffers (torch CUDA tensors or raw addresses).  `status`: an int32 on
+    the device that a bounded wait which runs out sets a bit of (read it with ``check_status``)."""
+    args = _quant_args(x, q, scale, weight, residual, up, sum_out, stream)
+    L = _lib or lib()
+    rc = L.frisk_b200_quant_run(C.byref(desc), args) if status is None else L.frisk_b200_quant_run_status(C.byref(desc), args, _ptr(status))
     if rc:
         _check(rc, "quant_run")
 

@@ -410,8 +410,12 @@ typedef struct frisk_quant_args {
  * same pointer and pitch).
  */
 int frisk_b200_quant_run(const frisk_quant_desc* desc, const frisk_quant_args* args);
+/* The same with a status word: many gated rows are streamed through shared memory with bounded waits, and
+ * a wait that runs out ORs a non-zero code into *device_status (one int32 in device memory; NULL: not
+ * reported), as in frisk_b200_gemm_run.  The rows it could not finish have NaN scales and zeros for q. */
+int frisk_b200_quant_run_status(const frisk_quant_desc* desc, const frisk_quant_args* args, int32_t* device_status);
 /* The same on HOST buffers (args->stream is not used): allocates, copies in, runs, copies q, scale
- * and sum_out back, synchronises. */
+ * and sum_out back, synchronises.  FRISK_ERR_DEVICE_TIMEOUT if a wait ran out. */
 int frisk_b200_quant_run_host(const frisk_quant_desc* desc, const frisk_quant_args* args);
 
 /* ---- layout mapping ------------------------------------------------------------------- */

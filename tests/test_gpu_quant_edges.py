@@ -209,3 +209,49 @@ def test_infinite_gates(cols, q_type):
     assert np.isposinf(s[0]) and np.isnan(s[1:3]).all() and not q[:3].any()
     v, _ = ref.ref_quant(x[3:], W.F32, "silu_mul")
     check_q(q[3:], s[3:], v, "silu_mul", q_type)
+
+
+@pytest.mark.parametrize("rows,cols,in_type", [(4500, 4096, W.BF16), (1100, 16384, W.BF16), (1500, 12008, W.F16), (800, 28672, W.BF16)],
+                         ids=["4500x4096", "1100x16384", "1500x12008", "800x28672"])
+def test_streamed_rows_report_a_wait_that_runs_out(rows, cols, in_type):
+    """With no time to wait the teams give up on rows whose copies have not landed: the status word says
+    so, those rows have NaN scales and zeros, and the launches after it are as ever."""
+    import ctypes
+    import torch
+    dev = torch.device("cuda:0")
+    limit = R.lib().frisk_internal_quant_wait_cycles
+    limit.argtypes, limit.restype = [ctypes.c_int64], ctypes.c_int64
+    dt = torch.bfloat16 if in_type == W.BF16 else torch.float16
+    x = torch.randn((rows, 2 * cols), generator=torch.Generator(device=dev).manual_seed(cols), device=dev).to(dt)
+    desc = R.quant_desc(rows, cols, in_type, W.I8, "silu_mul")
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def run():
+        q = torch.full((rows, cols), 0x5A, dtype=torch.int8, device=dev)
+        s = torch.full((rows,), 7.0, device=dev)
+        torch.cuda.synchronize()
+        R.quant_run(desc, x, q, s, stream=torch.cuda.current_stream().cuda_stream, status=status)
+        torch.cuda.synchronize()
+        return q, s
+
+    want_q, want_s = run()
+    R.check_status(status)
+    before = limit(0)
+    try:
+        q, s = run()
+        with pytest.raises(R.FriskError) as e:
+            R.quant_host(x.view(torch.int16).cpu().numpy().view(W.storage_numpy_dtype(in_type)), in_type, W.I8, "silu_mul")
+        assert e.value.code == -6
+    finally:
+        limit(before)
+    assert before == 1 << 29
+    with pytest.raises(R.FriskError) as e:
+        R.check_status(status)
+    assert e.value.code == -6 and "0x10" in str(e.value)
+    lost = torch.isnan(s)
+    assert bool(lost.any()) and not bool(q[lost].any())
+    assert torch.equal(q[~lost], want_q[~lost]) and torch.equal(s[~lost], want_s[~lost])
+    status.zero_()
+    again_q, again_s = run()
+    R.check_status(status)
+    assert torch.equal(again_q, want_q) and torch.equal(again_s, want_s)
