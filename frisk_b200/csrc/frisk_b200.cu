@@ -1721,12 +1721,30 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
   }
 
   // operands with an odd row pitch are copied into the front of the workspace first
-  const void *A0 = A, *B0 = B;
   const size_t repack_bytes = pl->repack_a_bytes + pl->repack_b_bytes;
   const frisk_gemm_desc& k = pl->kd;
   if (repack_bytes) {
     if (!workspace || args->workspace_bytes < pl->ws_bytes) return FRISK_ERR_WORKSPACE;
     if ((uintptr_t)workspace % 16) return FRISK_ERR_MISALIGNED;
+  }
+  // (a copy starts on a 16-byte boundary whatever its source does; what the run comes to is settled before
+  // anything is launched)
+  const bool ptr_aligned = (pl->repack_a_bytes || (uintptr_t)A % 16 == 0) && (pl->repack_b_bytes || (uintptr_t)B % 16 == 0);
+  if ((args->n_peers > 0 || d.row_reduce) && !(whole_tile_tc && ptr_aligned)) {
+    g_last_error = "peer copies of C and the fused row reduce exist only in the whole-tile "
+                   "tensor-core kernels (16-byte aligned A and B; a plan that splits K is kept to "
+                   "whole tiles by desc.k_split = -1)";
+    return FRISK_ERR_UNSUPPORTED;
+  }
+  if (pl->info.kernel != FRISK_KERNEL_SIMT && !ptr_aligned) {
+    // TMA needs 16-byte aligned bases; the run still gives the right answer, about 100x slower,
+    // so it is counted (plan_info.cuda_core_runs) and noted where the caller can read it
+    ++pl->simt_fallback_runs;
+    g_last_error = "A or B is not 16-byte aligned: this run used the CUDA-core kernel";
+  }
+  if (pl->info.kernel == FRISK_KERNEL_SIMT || !ptr_aligned)
+    return launch_simt(d, A, B, C, sa, sb, st);  // the CUDA-core kernel has no alignment rule
+  if (repack_bytes) {
     const int es = elem_size(d.a_type);
     char* w = static_cast<char*>(workspace);
     RepackJob ja{}, jb{};   // copies; transposes go at once
@@ -1757,21 +1775,6 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
     }
     workspace = w + repack_bytes;   // what follows is the kernels' own scratch
   }
-  const bool ptr_aligned = ((uintptr_t)A % 16 == 0) && ((uintptr_t)B % 16 == 0);
-  if ((args->n_peers > 0 || d.row_reduce) && !(whole_tile_tc && ptr_aligned)) {
-    g_last_error = "peer copies of C and the fused row reduce exist only in the whole-tile "
-                   "tensor-core kernels (16-byte aligned A and B; a plan that splits K is kept to "
-                   "whole tiles by desc.k_split = -1)";
-    return FRISK_ERR_UNSUPPORTED;
-  }
-  if (pl->info.kernel != FRISK_KERNEL_SIMT && !ptr_aligned) {
-    // TMA needs 16-byte aligned bases; the run still gives the right answer, about 100x slower,
-    // so it is counted (plan_info.cuda_core_runs) and noted where the caller can read it
-    ++pl->simt_fallback_runs;
-    g_last_error = "A or B is not 16-byte aligned: this run used the CUDA-core kernel";
-  }
-  if (pl->info.kernel == FRISK_KERNEL_SIMT || !ptr_aligned)
-    return launch_simt(d, A0, B0, C, sa, sb, st);  // the CUDA-core kernel has no alignment rule
   if (pl->info.kernel == FRISK_KERNEL_I8_ROWS) return launch_i8_rows(pl, A, B, C, sa, sb, st);
 
   const bool swap = pl->info.kernel == FRISK_KERNEL_SKINNY;
