@@ -493,9 +493,9 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
   // The area is reserved either way: the element-wise path of a C without 16-byte alignment goes
   // through it too.
   // desc.epilogue = 4 on a CTA-pair plan: TMA tensor stores out of two staging buffers per warp
-  // (needs rows of C that start on 16-byte boundaries, like every tensor map, and that end on them: the
-  // hardware clips a store at 16-byte units, so of a row of 2037 bf16 elements at a pitch of 2040 it would
-  // write the three elements of padding too).
+  // (needs rows of C that start on 16-byte boundaries, like every tensor map.  The hardware clips a store at
+  // 16-byte units: of a row of 2037 bf16 elements at a pitch of 2040 it would write the three elements of
+  // padding too.  So the maps describe whole units, and what is left of a row goes by itself).
   // Taken by default when K is short (at most 32 k-blocks): the epilogue of a tile then takes
   // longer than its main loop, and the tensor stores need a fraction of the instructions
   // (measured, bf16 8192 x 8192 x K: K = 256 58.6 -> 41.4 us, K = 512 65.3 -> 54.3 us, equal from
@@ -507,7 +507,7 @@ void plan_tcgen05(frisk_gemm_plan* pl, bool swap, bool pair, int cluster_try = 0
                                     (int64_t)(d.num_ctas > 1 ? std::min(d.num_ctas, pl->sm_count) : pl->sm_count);
   const bool want_tma = d.epilogue == 4 || (d.epilogue == 0 && (short_k || one_wave));
   const bool epi_tma = pair && !planes && !pcl && !pl->tf32 && want_tma &&
-                       (d.ldc * (int64_t)elem_size(d.c_type)) % 16 == 0 && (d.N * (int64_t)elem_size(d.c_type)) % 16 == 0;
+                       (d.ldc * (int64_t)elem_size(d.c_type)) % 16 == 0;
   const size_t epi_bytes = (split || pcl) ? 0 : (epi_tma ? 2 : 1) * frisk::kEpiStageBytes;
   // (the other pairs' images of the rows a CTA owns: [pair][row of the share][tile_n + 4] fp32)
   if (pcl) red_bytes = ((size_t)(pair_cluster - 1) * (128 / pair_cluster) * (g.tile_n + 4) * sizeof(float) + 1023) / 1024 * 1024;
@@ -659,7 +659,7 @@ int ensure_dyn_smem(Kern kern, int device) {
   return FRISK_OK;
 }
 template <typename TC, bool kSplit, bool kTf32 = false, bool kInt = false> struct OneCtaKernelTag {};
-template <typename TC, bool kTf32 = false, bool kInt = false> struct PairKernelTag {};
+template <typename TC, bool kTf32 = false, bool kInt = false, bool kTails = false> struct PairKernelTag {};
 
 template <typename TC, bool kSplit, bool kTf32 = false, bool kInt = false>
 int launch_tcgen05_ts(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
@@ -738,10 +738,10 @@ int launch_tcgen05_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream
   return g.split_mode ? launch_tcgen05_ts<TC, true>(pl, g, st) : launch_tcgen05_ts<TC, false>(pl, g, st);
 }
 
-template <typename TC, bool kTf32 = false, bool kInt = false>
+template <typename TC, bool kTf32 = false, bool kInt = false, bool kTails = false>
 int launch_pair_tf(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
-  auto kern = frisk::gemm_tcgen05_pair_kernel<TC, kTf32, kInt>;
-  if (int rc = ensure_dyn_smem<PairKernelTag<TC, kTf32, kInt>>(kern, pl->device)) return rc;
+  auto kern = frisk::gemm_tcgen05_pair_kernel<TC, kTf32, kInt, kTails>;
+  if (int rc = ensure_dyn_smem<PairKernelTag<TC, kTf32, kInt, kTails>>(kern, pl->device)) return rc;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof cfg);
   cfg.gridDim = dim3((unsigned)pl->info.num_ctas, 1, 1);
@@ -763,7 +763,10 @@ int launch_pair_tf(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t
 
 template <typename TC>
 int launch_pair_t(frisk_gemm_plan* pl, const frisk::GemmParams& g, cudaStream_t st) {
-  return pl->d.a_type == FRISK_DT_I8 ? launch_pair_tf<TC, false, true>(pl, g, st) : launch_pair_tf<TC>(pl, g, st);
+  const bool tails = g.epi_staged == 3u && pl->d.N * (int64_t)sizeof(TC) % 16 != 0;
+  if (pl->d.a_type == FRISK_DT_I8)
+    return tails ? launch_pair_tf<TC, false, true, true>(pl, g, st) : launch_pair_tf<TC, false, true>(pl, g, st);
+  return tails ? launch_pair_tf<TC, false, false, true>(pl, g, st) : launch_pair_tf<TC>(pl, g, st);
 }
 
 // The CTA-pair kernel with K split over the pairs of a cluster: one cluster of 2 x cluster_k CTAs
@@ -1813,12 +1816,13 @@ int frisk_b200_gemm_run_ex(frisk_gemm_plan* pl, const frisk_gemm_run_args* args)
     if (!g.c_vec_ok) {
       g.epi_staged = 1u;  // a base off the 16-byte grid: this run stores without TMA
     } else {
-      // one map per destination: [rows of this plan, N] of C's type at pitch ldc, boxes of
-      // 32 rows x 128 bytes in the 128-byte swizzle the staging buffers are written in
+      // one map per destination: [rows of this plan, the whole 16-byte units of N] of C's type at pitch
+      // ldc, boxes of 32 rows x 128 bytes in the 128-byte swizzle the staging buffers are written in
+      const int64_t units = d.N - d.N % (16 / elem_size(d.c_type));
       for (int q = 0; q <= args->n_peers; ++q) {
         void* dst = q == 0 ? C : args->peer_c[q - 1];
         if (dst == pl->cached_c[q]) continue;
-        if (int rc = encode_store_map(&pl->c_maps.m[q], dst, d.c_type, d.M, d.N, d.ldc)) return rc;
+        if (int rc = encode_store_map(&pl->c_maps.m[q], dst, d.c_type, d.M, units, d.ldc)) return rc;
         pl->cached_c[q] = dst;
       }
     }

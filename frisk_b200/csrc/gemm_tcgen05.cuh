@@ -497,6 +497,23 @@ __device__ __noinline__ void staged_rows_out(TC* C, void* const* peers, uint32_t
   }
 }
 
+// What a tensor store leaves of a row that ends off 16-byte units: the elements behind the last unit, one row
+// per lane (1 to 7 elements), from the staging buffer `buf`, where the lane has just written them.
+template <typename TC>
+__device__ __noinline__ void staged_tails_out(TC* C, void* const* peers, uint32_t n_peers, int64_t ldc, uint32_t rows,
+                                              uint32_t cols, uint32_t buf, uint32_t lane, uint32_t warp_row0, uint32_t col0) {
+  const uint32_t row = warp_row0 + lane;
+  if (row >= rows) return;
+#pragma unroll 1
+  for (uint32_t c = cols - cols % (16u / (uint32_t)sizeof(TC)); c < cols; ++c) {
+    const TC v = *staged_elem<TC>(buf, lane, c - col0, 7u);
+    const int64_t off = (int64_t)row * ldc + c;
+    C[off] = v;
+#pragma unroll 1
+    for (uint32_t q = 0; q < n_peers; ++q) reinterpret_cast<TC*>(peers[q])[off] = v;
+  }
+}
+
 // Whole staged rows (128 bytes each) to a C whose rows do not start on 16-byte boundaries.  Only the
 // integer kernels have these two: their mere presence cost the others' short-K shapes up to 10 %.
 // (int8, element by element -> here: bf16 C 4096 x 4097 x 4096 97 -> 52 us, 4096 x 4100 x 4096 98 -> 51 us,
@@ -556,7 +573,9 @@ __device__ __noinline__ void staged_rows_halves(char* dst0, int64_t pitch, uint3
 //   direct: every thread writes its own row piece (16-byte stores at row stride);
 //   a C without 16-byte alignment, or the chunk that crosses the last column, goes element-wise.
 // `stage` is the warp's staging area (shared-memory address), `warp_row0` the D row of lane 0.
-template <typename TC, int NC, bool kInt>
+// kTails: rows that leave by tensor stores may end off 16-byte units (kernels of their own: in the others
+// these few lines cost 8192 x 8192 x 256 bf16 39.2 -> 40.8 us).
+template <typename TC, int NC, bool kInt, bool kTails>
 __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint32_t stage,
                                                uint32_t lane, uint32_t warp_row0, uint32_t col0,
                                                const uint32_t (&acc)[NC], float& red) {
@@ -673,14 +692,18 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
     for (int v0 = 0; v0 < kVecs; ++v0) st_shared_v4(staged_chunk(buf, lane, (uint32_t)v0, 7u), out[v0].u);
     ptx::fence_proxy_async_smem();   // the writes above, made visible to the TMA unit
     __syncwarp();
+    // (the tensor maps describe whole 16-byte units of a row)
+    const uint32_t units = kTails ? p.cols - p.cols % (uint32_t)kPerVec : p.cols;
     if (lane == 0) {
-      if (warp_row0 < p.rows && col0 < p.cols) {
+      if (warp_row0 < p.rows && col0 < units) {
 #pragma unroll 1
         for (uint32_t q = 0; q <= x.n_peers; ++q)
           ptx::tma_store_2d(x.c_maps + q, buf, (int32_t)col0, (int32_t)warp_row0);
       }
       ptx::bulk_commit_group();   // one group per chunk, empty or not: the waits count groups
     }
+    if (kTails && !full && col0 < p.cols)
+      staged_tails_out<TC>(C, x.peers, x.n_peers, p.ldc, p.rows, p.cols, buf, lane, warp_row0, col0);
     return;
   }
 #pragma unroll
@@ -716,7 +739,7 @@ __device__ __forceinline__ void epilogue_chunk(const EpiArgs& p, EpiExt& x, uint
 // The warp's 32 rows of one work item: `cols_item` columns from D column `col0`, accumulator
 // rows at tensor-memory address `t_row`.  Columns are taken 128 bytes of C at a time; the
 // tensor-memory loads of a piece are issued together and waited for once.
-template <typename TC, bool kInt = false>
+template <typename TC, bool kInt = false, bool kTails = false>
 __device__ __forceinline__ void epilogue_item(const EpiArgs& ep, EpiExt& ex, uint32_t stage,
                                               uint32_t lane, uint32_t warp_row0, uint32_t col0,
                                               uint32_t cols_item, uint32_t t_row, float& red) {
@@ -729,7 +752,7 @@ __device__ __forceinline__ void epilogue_item(const EpiArgs& ep, EpiExt& ex, uin
       ptx::tmem_ld_32x32b_x32(t_row + cc + 32u * h, reinterpret_cast<uint32_t(&)[32]>(v[32 * h]));
     ptx::tmem_ld_wait();
     if constexpr (!std::is_same_v<TC, int32_t>) sums_to_f32<kInt>(v);
-    epilogue_chunk<TC, CH, kInt>(ep, ex, stage, lane, warp_row0, col0 + cc, v, red);
+    epilogue_chunk<TC, CH, kInt, kTails>(ep, ex, stage, lane, warp_row0, col0 + cc, v, red);
   }
 }
 

@@ -50,7 +50,8 @@ __device__ __forceinline__ PairItem pair_item(uint32_t i, uint32_t narrow_from, 
 
 // kTf32 (C fp32 only) issues kind::tf32 MMAs on fp32 operand tiles: the 3xTF32 plan of fp32 GEMMs.
 // kInt issues kind::i8 MMAs (TC = int32_t: the planes of an integer product split over K).
-template <typename TC, bool kTf32 = false, bool kInt = false>
+// kTails: tensor stores of rows that end off 16-byte units.
+template <typename TC, bool kTf32 = false, bool kInt = false, bool kTails = false>
 __global__ void __launch_bounds__(kGemmThreads, 1)
 gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                          const __grid_constant__ CUtensorMap tmap_b,
@@ -349,7 +350,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
       const uint32_t warp_row0 = tr * 256u + rank * 128u + quarter * 32u;
       const uint32_t t_row = tmem_base + ((quarter * 32u) << 16) + acc * tile_n;
       float red = fold_identity(rf.kind);
-      epilogue_item<TC, kInt>(ep, ex, stage_area, lane, warp_row0, col0, cols_item, t_row, red);
+      epilogue_item<TC, kInt, kTails>(ep, ex, stage_area, lane, warp_row0, col0, cols_item, t_row, red);
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive_cluster(leader_acc_empty0 + 8 * acc);
