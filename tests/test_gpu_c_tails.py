@@ -60,3 +60,24 @@ def test_every_end_of_a_32_bit_row(ab, N, clear):
 def test_copies_get_the_same_rows(ct, M, N):
     import torch
     case(torch, M, N, 80, 2048, W.BF16, ct, peers=2)
+
+
+@pytest.mark.parametrize("kind", ["max", "add"])
+@pytest.mark.parametrize("ab,ct,N", [(W.BF16, W.BF16, 1021), (W.I8, W.F32, 1022), (W.I8, W.BF16, 133)], ids=["bf16", "i8-f32", "i8-bf16"])
+def test_row_reduce_of_such_rows(ab, ct, N, kind):
+    import torch
+    dev = torch.device("cuda:0")
+    M, K, ldc = 520, 64, 1024
+    types = {k: getattr(torch, v) for k, v in TYPES.items()}
+    gen = torch.Generator(device=dev).manual_seed(N)
+    a, b = (torch.randint(-1, 2, (n, K), generator=gen, device=dev).to(types[ab]) for n in (M, N))
+    c, dst = torch.full((M, ldc), 7.0, dtype=types[ct], device=dev), torch.zeros(M, dtype=types[ct], device=dev)
+    plan = R.GemmPlan(M, N, K, ab, ct, transB=True, ldc=ldc, epilogue=4, row_reduce=kind)
+    assert plan.info["kernel_name"] == "tcgen05_pair"
+    ws = torch.empty(max(16, plan.workspace_bytes), dtype=torch.uint8, device=dev)
+    plan.run_ex(a, b, c, workspace=ws, stream=torch.cuda.current_stream().cuda_stream, row_reduce_dst=dst)
+    torch.cuda.synchronize()
+    plan.close()
+    prod = a.double() @ b.double().T   # whole numbers up to 64: exact in every type, and so is a row's sum before its rounding
+    assert torch.equal(c[:, :N].double(), prod) and bool((c[:, N:] == 7).all())
+    assert torch.equal(dst, (prod.amax(1) if kind == "max" else prod.sum(1)).to(types[ct]))
