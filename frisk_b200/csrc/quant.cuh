@@ -166,11 +166,27 @@ __device__ __forceinline__ Factor row_factor(float sum_sq, uint32_t max_bits, in
   if (tiny) f = {rstd * (low ? 0x1p30f : 0x1p126f), 0.f, up};
   return f;
 }
+// A product r = v * (hi + lo) that fp32's rounding may have put on a border between two 8-bit numbers: an
+// odd number of at most 8 bits times a power of two, its lower 16 bits zero.  What the rounding took away
+// decides then: at least 2^-32 of r where v Q / max |v| is not that border (a quotient of 24-bit numbers
+// times Q), below 2^-45 where it is (hi + lo is good to 2^-46).  r goes to the neighbour on that side.
+__device__ __forceinline__ bool maybe_border(float r) { return (__float_as_uint(r) & 0xffffu) == 0; }
+__device__ __forceinline__ float off_border(float r, float v, float hi, float lo) {
+  const float rest = fmaf(v, lo, fmaf(v, hi, -r));
+  if (!maybe_border(r) || !(fabsf(rest) > fabsf(r) * 0x1p-40f) || !(fabsf(hi) > 0x1p-90f)) return r;   // (a smaller lo has too few bits)
+  return __uint_as_float(__float_as_uint(r) + ((rest < 0.f) == (r < 0.f) ? 1u : 0xffffffffu));
+}
+// fp32 values as they are: q is the exact rounding.  (The other kinds' v carries roundings of its own; for
+// 16-bit values no quotient that is not a border comes as near to one.)
+template <typename TIn, int KIND>
+constexpr bool kExactQ = sizeof(TIn) == 4 && KIND == FRISK_QUANT_PLAIN;
 // v * up * (hi + lo), to 2^-24 of it: exact where that is an fp32 number.
+template <bool kExact>
 __device__ __forceinline__ float times(float v, Factor f) {
   if (f.hi == 0.f) return 0.f;
   v *= f.up;
-  return fmaf(v, f.hi, v * f.lo);
+  const float r = fmaf(v, f.hi, v * f.lo);
+  return kExact ? off_border(r, v, f.hi, f.lo) : r;
 }
 
 // Every kernel here is a programmatic dependent launch: it may be scheduled while the kernel before it
@@ -289,7 +305,7 @@ __global__ void __launch_bounds__(256) quant_rows_generic_kernel(const Params p)
     // sum_out may be x or the residual: an element is written by the thread that has just read it
     for (int64_t c = threadIdx.x; c < p.cols; c += 256) {
       const float v = value(c, &h);
-      q[c] = encode8(times(v, f), p.q_type);
+      q[c] = encode8(times<kExactQ<TIn, KIND>>(v, f), p.q_type);
       if (is_norm(KIND) && so) so[c] = from_float<TIn>(h);
     }
     __syncthreads();   // the shared arrays are written again by the next row
@@ -502,7 +518,7 @@ __device__ __forceinline__ void group_values(const Eight<TIn>& x, const Eight<TI
 }
 
 // g times the row's factor, in place.
-template <int NV>
+template <bool kExact, int NV>
 __device__ __forceinline__ void multiply(f2 (&g)[NV][4], Factor f) {
   if (f.up != 1.f || f.hi == 0.f) {
 #pragma unroll
@@ -512,9 +528,22 @@ __device__ __forceinline__ void multiply(f2 (&g)[NV][4], Factor f) {
   }
   const f2 hi = pack2(f.hi), lo = pack2(f.lo);
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    f2 r[4];
+    uint32_t low = 0xffffffffu;   // the least lower halves, of even and odd elements
 #pragma unroll
-    for (int j = 0; j < 4; ++j) g[i][j] = fma2(g[i][j], hi, mul2(g[i][j], lo));
+    for (int j = 0; j < 4; ++j) {
+      r[j] = fma2(g[i][j], hi, mul2(g[i][j], lo));
+      if (kExact) low = __vminu2(low, __byte_perm(__float_as_uint(lo2(r[j])), __float_as_uint(hi2(r[j])), 0x5410));
+    }
+    if (kExact && ((low & 0xffffu) == 0 || (low & 0xffff0000u) == 0)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        r[j] = pack2(off_border(lo2(r[j]), lo2(g[i][j]), f.hi, f.lo), off_border(hi2(r[j]), hi2(g[i][j]), f.hi, f.lo));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[i][j] = r[j];
+  }
 }
 
 // Sum and maximum over the `wpr` warps of each of the CTA's rows, in every thread (a CTA barrier).
@@ -593,7 +622,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
   if constexpr (KIND == kNormAnyEps) {
     if (small_norm(sum, mx, p)) return small_norm_row<TIn, TW>(p, r);   // (the CTA has one row)
   }
-  multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  multiply<kExactQ<TIn, KIND>, NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
   uint2 bytes[NV];
   encode_groups<NV>(g, p.q_type, bytes);
@@ -664,7 +693,7 @@ __global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
 #pragma unroll 2
     for (int i = t; i < groups; i += 1024) {
       values(8 * (int64_t)i, true, sums, top);
-      multiply<1>(g, f);
+      multiply<kExactQ<TIn, KIND>, 1>(g, f);
       uint2 bytes[1];
       encode_groups<1>(g, p.q_type, bytes);
       *reinterpret_cast<uint2*>(q + 8 * (int64_t)i) = bytes[0];
@@ -889,7 +918,7 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
     store_sum();   // (the row's reads are behind the fold)
   }
   if (!live) return;
-  multiply<NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+  multiply<kExactQ<TIn, KIND>, NV>(g, row_factor<KIND>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
   uint2 bytes[NV];
   encode_groups<NV>(g, p.q_type, bytes);
   uint32_t qw[NV][2];
@@ -1054,7 +1083,7 @@ __global__ void __launch_bounds__(1024, 1) quant_gated_stream_kernel(const Param
     if (t == 0 && j + stages < n) fetch(j + stages, stage);
     mx = lane < wpr ? s_max[buf][team * wpr + lane] : 0u;
     warp_fold<FRISK_QUANT_SILU_MUL>(sum, mx);
-    multiply<NV>(g, row_factor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
+    multiply<false, NV>(g, row_factor<FRISK_QUANT_SILU_MUL>(sum, mx, p.cols, p.eps, p.q_type, t == 0, p.scale + r));
     uint8_t* q = static_cast<uint8_t*>(p.q) + r * p.ldq;
     uint2 eight[NV];
     encode_groups<NV>(g, p.q_type, eight);

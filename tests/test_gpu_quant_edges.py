@@ -59,6 +59,35 @@ def test_ties_of_16_bit_rows_fall_as_defined(rows, cols, in_type, q_type):
     assert (np.abs(s - want) <= 2.0 ** -24 * want).all()
 
 
+def borders(q_type):
+    """The numbers half way between two neighbours of an 8-bit type (positive)."""
+    codes = np.arange(256, dtype=np.uint8).view(W.storage_numpy_dtype(q_type))
+    with np.errstate(invalid="ignore"):
+        grid = W.decode(codes, q_type).astype(np.float64)
+    grid = np.unique(grid[np.isfinite(grid) & (grid >= 0) & (grid <= W.QUANT_MAX[q_type])])
+    return (grid[1:] + grid[:-1]) / 2
+
+
+@pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
+@pytest.mark.parametrize("rows,cols", [(64, 64), (700, 1024), (700, 1001), (40, 3001), (3, 40000), (3, 40001)])
+def test_fp32_rows_next_to_borders_round_exactly(rows, cols, q_type):
+    """fp32 rows as they are, with most elements within a few of fp32's steps of a border between two 8-bit
+    numbers: q is the rounding of the exact v Q / max |v|, without any allowance.  float64 decides that
+    exactly too: v Q is exact in it, and a quotient that is not a border differs from one by 2^-32 at least."""
+    rng = np.random.default_rng([8, rows, cols])
+    top = rng.uniform(1, 2, (rows, 1)).astype(np.float32) * np.exp2(rng.integers(-60, 60, (rows, 1))).astype(np.float32)
+    at = rng.choice(borders(q_type), (rows, cols)) * top.astype(np.float64) / W.QUANT_MAX[q_type]
+    x = at.astype(np.float32)
+    x = (x.view(np.int32) + rng.integers(-2, 3, x.shape)).astype(np.int32).view(np.float32)
+    x = np.clip(x * rng.choice([-1, 1], x.shape).astype(np.float32), -top, top)
+    x[:, cols // 2] = top[:, 0]
+    t = x.astype(np.float64) * W.QUANT_MAX[q_type] / top.astype(np.float64)
+    q, s = R.quant_host(x, W.F32, q_type)
+    got = W.decode(q, q_type).astype(np.float64)
+    bad = got != ref.round8(t, q_type)
+    assert not bad.any(), f"{int(bad.sum())} of {bad.size} values, first at {tuple(np.argwhere(bad)[0])}"
+
+
 @pytest.mark.parametrize("q_type", Q_TYPES, ids=ids)
 @pytest.mark.parametrize("cols", [512] + WIDTHS)
 def test_rows_whose_squares_overflow_have_zeros_beside_their_scale(cols, q_type):
