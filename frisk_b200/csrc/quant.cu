@@ -102,9 +102,11 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
   p.late_sum = small_norms && p.sum_out && (p.sum_out == p.x || p.sum_out == p.other);
   const int64_t groups = ceil_div(p.cols, 8);
   if constexpr (KIND == FRISK_QUANT_SILU_MUL) {
-    // Streamed from two fillings of all SMs' rings on (bf16 / f16, in registers -> streamed: 67 MB of
-    // input 19.2 -> 19.2 us, 98 MB 30.8 -> 27.4, 134 MB 39.1 -> 34.7, 537 MB 73.0 -> 61.6; 33 MB 10.0 ->
-    // 13.0, 39 MB 14.1 -> 14.9).
+    // Streamed from two fillings of all SMs' rings on, 68 MB of input.  In registers -> streamed, us: bf16 of
+    // 8192 columns 50 MB 12.6 -> 14.9, 67 MB 15.9 -> 17.3, 134 MB 29.5 -> 29.7, 268 MB 54.9 -> 54.3; of 16384
+    // columns 50 MB 14.2 -> 16.1, 67 MB 17.3 -> 18.0, 134 MB 31.1 -> 30.1, 268 MB 59.5 -> 54.9; with one
+    // team a CTA, 20480 columns, 34 MB 12.3 -> 12.8, 67 MB 22.9 -> 20.8, 268 MB 78.8 -> 64.7; fp32 of 8192 columns
+    // 67 MB 24.1 -> 20.3, 268 MB 58.0 -> 47.3.
     const size_t row = 2 * (size_t)p.cols * es;
     const int stages = (int)std::min<size_t>(frisk_quant::kMaxRowStages, kRingBytes / row);
     const int wpr = (int)ceil_div(groups, 32 * kMaxGroups);
@@ -119,10 +121,10 @@ cudaError_t launch(Params p, int device, int sms, cudaStream_t st) {
       return go(kern, sms, dim3(32 * wpr, teams), stages * row, p, st);
     }
   }
-  // Many rows: four groups a thread, the most loads in flight per warp that registers allow (off the
-  // 16-byte grid two, but of 16-bit rows as they are: 1023 x 5001 f16 norm 9.9 us with two, 12.2 with
-  // four; 8192 x 4095 bf16 as it is 34.6 and 29.9); few rows: one, so that a row is spread over as many
-  // threads as there are.
+  // Many rows: four groups a thread, for loads in flight (norms and gates of fp32 rows spill 80 - 210 bytes
+  // with them); off the 16-byte grid two, but of 16-bit rows as they are (1023 x 5001 f16
+  // norm with one, two, four: 15.5, 8.9, 11.1 us; 8192 x 4095 bf16 as it is 43.3, 35.8, 30.5).  Few rows: one, so
+  // that a row is spread over as many threads as there are.
   const bool few = p.rows < 2 * (int64_t)sms;
   int nv = few ? 1 : aligned || (es == 2 && KIND == FRISK_QUANT_PLAIN) ? kMaxGroups : 2;
   while (ceil_div(groups, 32 * nv) > 32) nv *= 2;

@@ -568,7 +568,7 @@ __device__ __forceinline__ void row_fold(float& sum, uint32_t& mx, float* s_sum,
 // For rows whose starts, in every buffer, allow 16-byte accesses (8 for q) and whose width is a
 // multiple of eight.  CTAs of more than one row (blockDim.y) fold them side by side.
 // kFull: every thread has all of its groups, of a row that exists (no bounds to test).
-// Bound by memory where rows are many: 8192 x 8192 bf16 norm with residual 75 - 78 us (470 MB, 0.92 - 0.95
+// Bound by memory where rows are many: 8192 x 8192 bf16 norm with residual 73 - 77 us (470 MB, 0.94 - 0.99
 // of the copy rate; two passes element by element 168 us), fp32 as it is 50 us (336 MB, 1.0; 96 us).
 // Few rows take one group per thread, since then the launch and the row's own latency are all there
 // is: 1 x 4096 norm 1.8 us.
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const Params p) {
 }
 
 // Rows wider than a CTA's registers hold, with the alignment of quant_rows_kernel: two passes over the
-// row, the second one from L2, a group of eight per thread and step (2048 x 53248 bf16 as it is: 91 us,
+// row, the second one from L2, a group of eight per thread and step (2048 x 53248 bf16 as it is: 89 us,
 // 273 element by element).  (h goes to sum_out in the second
 // pass: the first one may not yet have read its place.)
 template <typename TIn, typename TW, int KIND>
@@ -703,8 +703,8 @@ __global__ void __launch_bounds__(1024) quant_rows_wide_kernel(const Params p) {
 }
 
 // ---- the same for rows at any alignment and width -----------------------------------------------
-// Bound by instructions (40 per element, 52 when every element was accessed by itself): 1023 x 5001 f16
-// norm 9.1 us, 12.9 element by element; 2047 x 4095 bf16 out of rows of 6150 7.9 us.
+// What it takes is its instructions (35 per element, 52 when every element was accessed by itself): 1023 x
+// 5001 f16 norm 8.9 us, 12.9 element by element; 2047 x 4095 bf16 out of rows of 6150 8.1 us (20).
 // Memory is still touched in aligned words of 16 bytes (8 for q): a group that starts inside a word is
 // shifted together from the words it lies in, and a stored word from the end of one lane's group and
 // the start of the next one's.
@@ -932,9 +932,8 @@ __global__ void __launch_bounds__(1024) quant_rows_unaligned_kernel(const Params
 
 // ---- many gated rows: streamed through shared memory ---------------------------------------------
 // The gate costs enough arithmetic that rows in registers alternate between loading and computing
-// (4096 x 16384 bf16: 73 us at half the DRAM rate and 54 % of the issue slots; streamed 59 - 61 us; the
-// other kinds are faster in registers: norm 8192 x 8192 with residual 79 against 80 us, fp32 8192 x
-// 8192 as it is 50 against 55).
+// (4096 x 16384 bf16: 59.5 us; streamed 55 - 57 us; the other kinds are faster in registers: norm 8192 x
+// 8192 with residual 79 against 80 us, fp32 8192 x 8192 as it is 50 against 55).
 // One CTA per SM walks the rows blockIdx.x, + gridDim.x, ...; bulk copies bring them into a ring of
 // `stages` whole rows (both operands), several ahead of the arithmetic, so that the memory is read
 // without a pause while rows are folded, scaled and stored.  The CTA is blockDim.y teams of
